@@ -145,7 +145,7 @@ def _store(c, st, seed):
         src = st[x]
         full = torch.zeros((B, Hkv, cap) + tuple(src.shape[3:]), dtype=src.dtype, device=DEV)
         full[:, :, :T] = src
-        full = full.view((B, Hkv, nb, BLOCK) + tuple(src.shape[3:])).transpose(1, 2).reshape((B * nb, Hkv, BLOCK) + tuple(src.shape[3:]))
+        full = full.view((B, Hkv, nb, BLOCK) + tuple(src.shape[3:])).transpose(1, 2).reshape((B * nb, Hkv, BLOCK) + tuple(src.shape[3:])).contiguous()
         pool = torch.empty_like(full)
         pool[where] = full
         st[x] = pool
