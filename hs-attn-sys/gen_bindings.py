@@ -124,11 +124,11 @@ pub struct hs_kv_layout {
     pub prefill_split_workspace: *mut c_void,
     pub prefill_split_workspace_bytes: i64,
     pub prefill_key_splits: i32,
-    pub reserved0: i32,
+    pub attn_sinks: i32,
     pub prefill_shadow: *mut c_void,
     pub prefill_shadow_bytes: i64,
     pub prefill_shadow_tokens: i32,
-    pub reserved1: i32,
+    pub decode_window: i32,
 }
 
 #[repr(C)]

@@ -59,11 +59,11 @@ pub struct hs_kv_layout {
     pub prefill_split_workspace: *mut c_void,
     pub prefill_split_workspace_bytes: i64,
     pub prefill_key_splits: i32,
-    pub reserved0: i32,
+    pub attn_sinks: i32,
     pub prefill_shadow: *mut c_void,
     pub prefill_shadow_bytes: i64,
     pub prefill_shadow_tokens: i32,
-    pub reserved1: i32,
+    pub decode_window: i32,
 }
 
 #[repr(C)]
@@ -111,6 +111,12 @@ extern "C" {
     pub fn hs_decode_step_fp8(q: *const c_void, k_new: *const c_void, v_new: *const c_void, src_dtype: c_int, k_codes: *mut u8, v_codes: *mut u8, k_scales: *const f32, v_scales: *const f32, layout: *const hs_kv_layout, seq_lens: *const i32, out: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, b: i32, hq: i32, hkv: i32, d: i32, max_seq_len: i32, softmax_scale: f32, stream: hs_stream_t) -> c_int;
     pub fn hs_decode_step_fp8_prologue(q: *const c_void, k_new: *const c_void, v_new: *const c_void, prologue: *const hs_qk_prologue, k_codes: *mut u8, v_codes: *mut u8, k_scales: *const f32, v_scales: *const f32, layout: *const hs_kv_layout, seq_lens: *const i32, out: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, b: i32, hq: i32, hkv: i32, d: i32, max_seq_len: i32, softmax_scale: f32, stream: hs_stream_t) -> c_int;
     pub fn hs_decode_attn_phases(fmt_fp8: c_int, phases: c_int, q: *const c_void, k_codes: *const c_void, v_codes: *const c_void, k_scales: *const f32, v_scales: *const f32, layout: *const hs_kv_layout, seq_lens: *const i32, out: *mut c_void, workspace: *mut c_void, workspace_bytes: usize, b: i32, hq: i32, hkv: i32, d: i32, max_seq_len: i32, softmax_scale: f32, stream: hs_stream_t) -> c_int;
+    pub fn hs_decode_weights_workspace_bytes(b: i32, hq: i32, hkv: i32, d: i32, max_seq_len: i32) -> usize;
+    pub fn hs_decode_step_weights(fmt_fp8: c_int, q: *const c_void, k_new: *const c_void, v_new: *const c_void, src_dtype: c_int, k_codes: *mut c_void, v_codes: *mut c_void, k_scales: *mut f32, v_scales: *mut f32, layout: *const hs_kv_layout, seq_lens: *const i32, out: *mut c_void, weights_in: *const f32, weights_out: *mut f32, weights_stride: i64, workspace: *mut c_void, workspace_bytes: usize, b: i32, hq: i32, hkv: i32, d: i32, max_seq_len: i32, softmax_scale: f32, stream: hs_stream_t) -> c_int;
+    pub fn hs_attn_weights_workspace_bytes(b: i32, s: i32, hq: i32, hkv: i32, d: i32, max_seq_len: i32) -> usize;
+    pub fn hs_attn_weights(fmt_fp8: c_int, q: *const c_void, k_codes: *const c_void, k_scales: *const f32, layout: *const hs_kv_layout, positions: *const i32, start_pos: i32, weights_in: *const f32, weights_out: *mut f32, weights_stride: i64, workspace: *mut c_void, workspace_bytes: usize, b: i32, s: i32, hq: i32, hkv: i32, d: i32, max_seq_len: i32, softmax_scale: f32, stream: hs_stream_t) -> c_int;
+    pub fn hs_kv_evict_workspace_bytes(b: i32, hkv: i32, budget: i32, max_seq_len: i32) -> usize;
+    pub fn hs_kv_evict(fmt_fp8: c_int, k_codes: *const c_void, v_codes: *const c_void, k_scales: *const f32, v_scales: *const f32, layout: *const hs_kv_layout, seq_lens: *const i32, weights: *const f32, weights_stride: i64, k_codes_out: *mut c_void, v_codes_out: *mut c_void, k_scales_out: *mut f32, v_scales_out: *mut f32, layout_out: *const hs_kv_layout, seq_lens_out: *mut i32, weights_out: *mut f32, weights_out_stride: i64, kept: *mut i32, budget: i32, sinks: i32, recent: i32, workspace: *mut c_void, workspace_bytes: usize, b: i32, hkv: i32, d: i32, max_seq_len: i32, stream: hs_stream_t) -> c_int;
     pub fn hs_prefill_attn_int8(q: *const c_void, k_new: *const c_void, v_new: *const c_void, k_codes: *mut i8, v_codes: *mut i8, k_scales: *mut f32, v_scales: *mut f32, layout: *const hs_kv_layout, hist_len: i32, out: *mut c_void, b: i32, s: i32, hq: i32, hkv: i32, d: i32, softmax_scale: f32, quantize_on_write: c_int, stream: hs_stream_t) -> c_int;
     pub fn hs_prefill_attn_fp8(q: *const c_void, k_new: *const c_void, v_new: *const c_void, k_codes: *mut u8, v_codes: *mut u8, k_scales: *const f32, v_scales: *const f32, layout: *const hs_kv_layout, hist_len: i32, out: *mut c_void, b: i32, s: i32, hq: i32, hkv: i32, d: i32, softmax_scale: f32, quantize_on_write: c_int, stream: hs_stream_t) -> c_int;
     pub fn hs_prefill_attn_int8_ragged(q: *const c_void, k_new: *const c_void, v_new: *const c_void, k_codes: *mut i8, v_codes: *mut i8, k_scales: *mut f32, v_scales: *mut f32, layout: *const hs_kv_layout, hist_lens: *const i32, max_hist_len: i32, out: *mut c_void, b: i32, s: i32, hq: i32, hkv: i32, d: i32, softmax_scale: f32, quantize_on_write: c_int, stream: hs_stream_t) -> c_int;

@@ -29,6 +29,8 @@ EXPORTS = [
     "hs_decode_attn_int8_static", "hs_qk_prologue_apply", "hs_kv_quantize_int8_prologue", "hs_decode_step_int8_prologue", "hs_decode_step_fp8_prologue",
     "hs_deltanet_prepare", "hs_deltanet_gated_norm", "hs_deltanet_decode_layer", "hs_deltanet_forward_chunked", "hs_deltanet_forward_chunked_gated_norm", "hs_deltanet_prefill_layer", "hs_deltanet_prefill_layer_workspace_bytes", "hs_prefill_attn_int8_ragged", "hs_prefill_attn_fp8_ragged", "hs_deltanet_chunked_workspace_bytes",
     "hs_deltanet_chunked_gated_norm_workspace_bytes", "hs_prefill_attn_split_workspace_bytes", "hs_prefill_attn_split_workspace_init", "hs_prefill_shadow_bytes", "hs_prefill_shadow_init",
+    "hs_decode_weights_workspace_bytes", "hs_decode_step_weights", "hs_attn_weights_workspace_bytes", "hs_attn_weights",
+    "hs_kv_evict_workspace_bytes", "hs_kv_evict",
 ]
 
 
@@ -51,11 +53,11 @@ class KvLayout(ctypes.Structure):
         ("prefill_split_workspace", ctypes.c_void_p),
         ("prefill_split_workspace_bytes", ctypes.c_int64),
         ("prefill_key_splits", ctypes.c_int32),
-        ("reserved0", ctypes.c_int32),
+        ("attn_sinks", ctypes.c_int32),
         ("prefill_shadow", ctypes.c_void_p),
         ("prefill_shadow_bytes", ctypes.c_int64),
         ("prefill_shadow_tokens", ctypes.c_int32),
-        ("reserved1", ctypes.c_int32),
+        ("decode_window", ctypes.c_int32),
     ]
 
 
@@ -120,6 +122,12 @@ def lib():
         L.hs_prefill_shadow_bytes.argtypes = [ctypes.c_int32] * 4
         L.hs_prefill_attn_split_workspace_bytes.restype = ctypes.c_size_t
         L.hs_prefill_attn_split_workspace_bytes.argtypes = [ctypes.c_int32] * 5
+        L.hs_decode_weights_workspace_bytes.restype = ctypes.c_size_t
+        L.hs_decode_weights_workspace_bytes.argtypes = [ctypes.c_int32] * 5
+        L.hs_attn_weights_workspace_bytes.restype = ctypes.c_size_t
+        L.hs_attn_weights_workspace_bytes.argtypes = [ctypes.c_int32] * 6
+        L.hs_kv_evict_workspace_bytes.restype = ctypes.c_size_t
+        L.hs_kv_evict_workspace_bytes.argtypes = [ctypes.c_int32] * 4
         _lib = L
     return _lib
 
@@ -214,10 +222,11 @@ def kv_quantize_int8_prologue(k_src, v_src, prologue, k_codes, v_codes, k_scales
 
 
 def decode_step_prologue(q, k_new, v_new, prologue, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out,
-                         workspace, Hkv, max_seq_len, softmax_scale, fp8=False):
+                         workspace, Hkv, max_seq_len, softmax_scale, fp8=False, window=0, sinks=0):
     """decode_step (int8, or fp8 with calibrated scales) with the QK-norm and the rotation of q and k_new inside the
-    launch."""
+    launch.  window, sinks: as for decode_attn."""
     B, Hq, D = q.shape
+    layout.decode_window, layout.attn_sinks = window, sinks
     assert k_new.shape == (B, 1, Hkv, D) and k_new.is_contiguous() and v_new.is_contiguous()
     fn = lib().hs_decode_step_fp8_prologue if fp8 else lib().hs_decode_step_int8_prologue
     check(fn(_ptr(q), _ptr(k_new), _ptr(v_new), ctypes.byref(prologue), _ptr(k_codes), _ptr(v_codes), _ptr(k_scales),
@@ -255,8 +264,11 @@ def decode_workspace_bytes(B, Hq, Hkv, D, max_seq_len):
 
 
 def decode_attn(q, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, workspace, Hkv, max_seq_len,
-                softmax_scale, fp8=False, phases=3):
+                softmax_scale, fp8=False, phases=3, window=0, sinks=0):
+    """window: the newest token attends the last `window` cached tokens (0 = all) and the first `sinks` ones
+    (layout.decode_window, layout.attn_sinks)."""
     B, Hq, D = q.shape
+    layout.decode_window, layout.attn_sinks = window, sinks
     if phases != 3:
         fn0 = lib().hs_decode_attn_phases
         fn = lambda *a: fn0(int(fp8), int(phases), *a)
@@ -268,18 +280,22 @@ def decode_attn(q, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, 
              B, Hq, Hkv, D, ctypes.c_int32(max_seq_len), ctypes.c_float(softmax_scale), _stream()))
 
 
-def decode_attn_static(q, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, Hkv, max_seq_len, softmax_scale):
+def decode_attn_static(q, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, Hkv, max_seq_len, softmax_scale,
+                       window=0, sinks=0):
     """hs_decode_attn_int8 without a workspace argument: the split-K partials use the library's built-in scratch."""
     B, Hq, D = q.shape
+    layout.decode_window, layout.attn_sinks = window, sinks
     check(lib().hs_decode_attn_int8_static(_ptr(q), _ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales),
                                            ctypes.byref(layout), _ptr(seq_lens), _ptr(out), B, Hq, Hkv, D,
                                            ctypes.c_int32(max_seq_len), ctypes.c_float(softmax_scale), _stream()))
 
 
 def decode_step(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, workspace, Hkv,
-                max_seq_len, softmax_scale, fp8=False):
-    """Quantize-on-write of one new token per sequence (at seq_lens-1) + decode attention, one call."""
+                max_seq_len, softmax_scale, fp8=False, window=0, sinks=0):
+    """Quantize-on-write of one new token per sequence (at seq_lens-1) + decode attention, one call.  window, sinks: as
+    for decode_attn."""
     B, Hq, D = q.shape
+    layout.decode_window, layout.attn_sinks = window, sinks
     assert k_new.shape == (B, 1, Hkv, D) and k_new.is_contiguous() and v_new.is_contiguous()
     fn = lib().hs_decode_step_fp8 if fp8 else lib().hs_decode_step_int8
     check(fn(_ptr(q), _ptr(k_new), _ptr(v_new), _dtype_code(k_new), _ptr(k_codes), _ptr(v_codes), _ptr(k_scales),
@@ -289,9 +305,10 @@ def decode_step(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, layout, s
 
 
 def decode_step_rope(q, k_new, v_new, rope_sin, rope_cos, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out,
-                     workspace, Hkv, max_seq_len, softmax_scale):
+                     workspace, Hkv, max_seq_len, softmax_scale, window=0, sinks=0):
     """decode_step (int8) with q and k_new arriving unrotated; bf16 tables [rope_len, D/2]."""
     B, Hq, D = q.shape
+    layout.decode_window, layout.attn_sinks = window, sinks
     assert k_new.shape == (B, 1, Hkv, D) and k_new.is_contiguous() and v_new.is_contiguous()
     check(lib().hs_decode_step_int8_rope(_ptr(q), _ptr(k_new), _ptr(v_new), _ptr(rope_sin), _ptr(rope_cos),
                                          ctypes.c_int32(rope_sin.shape[0]), _ptr(k_codes), _ptr(v_codes),
@@ -299,6 +316,80 @@ def decode_step_rope(q, k_new, v_new, rope_sin, rope_cos, k_codes, v_codes, k_sc
                                          _ptr(out), _ptr(workspace),
                                          ctypes.c_size_t(workspace.numel() * workspace.element_size()), B, Hq, Hkv, D,
                                          ctypes.c_int32(max_seq_len), ctypes.c_float(softmax_scale), _stream()))
+
+
+def decode_weights_workspace_bytes(B, Hq, Hkv, D, max_seq_len):
+    return lib().hs_decode_weights_workspace_bytes(B, Hq, Hkv, D, max_seq_len)
+
+
+def _weights_rows(w_in, w_out, B, Hkv):
+    """Rows of accumulated weights [B, Hkv, stride]; returns the stride."""
+    for t in (w_in, w_out):
+        assert t is None or (t.is_contiguous() and t.shape[:2] == (B, Hkv) and str(t.dtype) == "torch.float32")
+    assert w_in is None or w_in.shape == w_out.shape
+    return w_out.shape[2]
+
+
+def decode_step_weights(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, weights_in, weights_out,
+                        workspace, Hkv, max_seq_len, softmax_scale, fp8=False, window=0, sinks=0):
+    """decode_step (decode_attn if k_new and v_new are None) and weights_out = weights_in + the softmax weights of the
+    step summed over the query heads of each kv-head.  weights: fp32 [B, Hkv, stride]; weights_in may be None (zeros) or
+    weights_out itself."""
+    B, Hq, D = q.shape
+    assert q.is_contiguous() and out.is_contiguous()
+    assert k_new is None or (k_new.shape == (B, 1, Hkv, D) and k_new.is_contiguous() and v_new.is_contiguous())
+    stride = _weights_rows(weights_in, weights_out, B, Hkv)
+    layout.decode_window, layout.attn_sinks = window, sinks
+    check(lib().hs_decode_step_weights(int(fp8), _ptr(q), _ptr(k_new), _ptr(v_new), HS_BF16 if k_new is None else _dtype_code(k_new),
+                                       _ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), ctypes.byref(layout),
+                                       _ptr(seq_lens), _ptr(out), _ptr(weights_in), _ptr(weights_out), ctypes.c_int64(stride),
+                                       _ptr(workspace), ctypes.c_size_t(workspace.numel() * workspace.element_size()),
+                                       B, Hq, Hkv, D, ctypes.c_int32(max_seq_len), ctypes.c_float(softmax_scale), _stream()))
+
+
+def attn_weights_workspace_bytes(B, S, Hq, Hkv, D, max_seq_len):
+    return lib().hs_attn_weights_workspace_bytes(B, S, Hq, Hkv, D, max_seq_len)
+
+
+def attn_weights(q, k_codes, k_scales, layout, weights_in, weights_out, workspace, Hkv, max_seq_len, softmax_scale,
+                 positions=None, start_pos=0, fp8=False, window=0, sinks=0):
+    """weights_out = weights_in + the softmax weights of the queries q [B, S, Hq, D] (at (positions[b] or 0) + start_pos + s)
+    over the cached keys, summed over queries and over the query heads of each kv-head."""
+    B, S, Hq, D = q.shape
+    assert q.is_contiguous() and str(q.dtype) == "torch.bfloat16"
+    assert positions is None or (str(positions.dtype) == "torch.int32" and positions.is_contiguous() and positions.numel() == B)
+    stride = _weights_rows(weights_in, weights_out, B, Hkv)
+    layout.prefill_window, layout.attn_sinks = window, sinks
+    check(lib().hs_attn_weights(int(fp8), _ptr(q), _ptr(k_codes), _ptr(k_scales), ctypes.byref(layout), _ptr(positions),
+                                ctypes.c_int32(start_pos), _ptr(weights_in), _ptr(weights_out), ctypes.c_int64(stride),
+                                _ptr(workspace), ctypes.c_size_t(workspace.numel() * workspace.element_size()),
+                                B, S, Hq, Hkv, D, ctypes.c_int32(max_seq_len), ctypes.c_float(softmax_scale), _stream()))
+
+
+def kv_evict_workspace_bytes(B, Hkv, budget, max_seq_len):
+    return lib().hs_kv_evict_workspace_bytes(B, Hkv, budget, max_seq_len)
+
+
+def kv_evict(cache, layout, seq_lens, weights, cache_out, layout_out, seq_lens_out, weights_out, workspace, budget, sinks,
+             recent, max_seq_len, kept=None, fp8=False):
+    """Keep `budget` tokens per (sequence, kv-head): the first `sinks`, the last `recent` and the heaviest of those between,
+    moved to the front in their order.  cache, cache_out: (k_codes, v_codes, k_scales, v_scales); passing the same tensors
+    and layout evicts in place.  weights, weights_out: fp32 [B, Hkv, stride] or None; kept: int32 [B, Hkv, budget] or None."""
+    B = seq_lens.numel()
+    codes = cache[0]
+    Hkv, D = codes.shape[1], codes.shape[3]
+    for t in (weights, weights_out, kept, seq_lens, seq_lens_out):
+        assert t is None or (t.is_contiguous() and t.element_size() == 4)
+    assert kept is None or kept.shape == (B, Hkv, budget)
+    for t in (weights, weights_out):
+        assert t is None or t.shape[:2] == (B, Hkv)
+    check(lib().hs_kv_evict(int(fp8), *[_ptr(t) for t in cache], ctypes.byref(layout), _ptr(seq_lens), _ptr(weights),
+                            ctypes.c_int64(weights.shape[2] if weights is not None else 0), *[_ptr(t) for t in cache_out],
+                            ctypes.byref(layout_out), _ptr(seq_lens_out), _ptr(weights_out),
+                            ctypes.c_int64(weights_out.shape[2] if weights_out is not None else 0), _ptr(kept),
+                            ctypes.c_int32(budget), ctypes.c_int32(sinks), ctypes.c_int32(recent), _ptr(workspace),
+                            ctypes.c_size_t(workspace.numel() * workspace.element_size()), B, Hkv, D,
+                            ctypes.c_int32(max_seq_len), _stream()))
 
 
 def prefill_split_workspace(B, S, Hq, Hkv, D, device="cuda:0"):
@@ -329,11 +420,12 @@ PREFILL_COLUMNS = 0  # default for prefill_attn's `columns` (tests set it to run
 
 def prefill_attn(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, layout, hist_len, out, softmax_scale,
                  quantize_on_write=True, fp8=False, hist_lens=None, columns=None, window=0, q_prologue=None,
-                 split_workspace=None, key_splits=0, shadow=None):
+                 split_workspace=None, key_splits=0, shadow=None, sinks=0):
     """Causal attention of S new tokens over [int8 or fp8 history | their own bf16 K/V]; optionally caches them.
     hist_lens (int32 device tensor [B]): rows at different positions; hist_len is then their upper bound.
     columns: 0 = the library's choice of workgroup width, 256 or 128 fixes it (layout.prefill_columns_hint).
-    window: sliding window of local layers (layout.prefill_window), 0 = none.
+    window: sliding window of local layers (layout.prefill_window), 0 = none; sinks: first tokens that stay visible
+    (layout.attn_sinks).
     q_prologue (QkPrologue): q arrives as projected and the launch normalises and rotates it
     (layout.prefill_q_prologue); k_new arrives normalised and rotated either way.
     split_workspace (uint8 device tensor from prefill_split_workspace()): lets a call with few query tiles split their
@@ -342,7 +434,7 @@ def prefill_attn(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, layout, 
     every call appends to and calls with history read instead of the codes (layout.prefill_shadow)."""
     B, S, Hq, D = q.shape
     layout.prefill_columns_hint = PREFILL_COLUMNS if columns is None else columns
-    layout.prefill_window = window
+    layout.prefill_window, layout.attn_sinks = window, sinks
     layout.prefill_q_prologue = ctypes.addressof(q_prologue) if q_prologue is not None else None
     if split_workspace is None and key_splits == 0 and PREFILL_KEY_SPLITS > 1:
         key = (B, S, Hq, k_new.shape[2], D)

@@ -170,7 +170,38 @@ struct DecodeArgs {
     const uint16_t *rope_sin, *rope_cos;
     int32_t rope_len, rotary_dim;
     NormSpec qnorm;  // optional QK-norm of q ahead of the rotation (the new token's K: nt.norm)
+    int32_t window, sinks;  // kMode >= 1: sliding window (0 = none) and the first tokens that stay visible
+    float *logits;          // kMode 2: scores in log2 units [B, Hq, logit_stride] by token on the visible line; -inf = not visible
+    int64_t logit_stride;
 };
+
+// Sliding window with sinks.  The query (the newest token, position L - 1) sees the tokens t >= wbegin and t < sinks.
+// Whole wavefront steps without a visible token are cut out: the steps that are left, laid end to end, are the "visible
+// line", and everything that splits work (chunks, items, partial slots) counts tokens on it.  The cut starts and ends at
+// multiples of the step, so a step lies inside one pool block as before; the steps at the cut's ends mask what is not
+// visible.  Every step of the line holds at least one visible token (a sink, or the window's first token or later).
+struct VisibleLine {
+    int wbegin;    // first token of the window
+    int cut, len;  // tokens [cut, cut + skip) are left out; len = tokens on the line
+    int skip;
+};
+__host__ __device__ inline VisibleLine visible_line(int L, int window, int sinks, int step) {
+    VisibleLine v = {0, 0, L, 0};
+    if (window <= 0 || L <= window) return v;
+    v.wbegin = L - window;
+    if (sinks >= v.wbegin) return v;
+    v.cut = (sinks + step - 1) / step * step;
+    const int first = v.wbegin / step * step;
+    if (first > v.cut) v.skip = first - v.cut;
+    v.len = L - v.skip;
+    return v;
+}
+// Longest visible line of sequences of at most max_seq_len tokens.
+static int visible_bound(int max_seq_len, int window, int sinks, int step) {
+    if (window <= 0) return max_seq_len;
+    const int64_t b = (int64_t)window + step - 1 + ((int64_t)sinks + step - 1) / step * step;
+    return (int)std::min<int64_t>(max_seq_len, b);
+}
 
 // Half-split rotary embedding of the query elements a lane holds, in bf16 arithmetic (every product and sum rounded
 // to bf16, as the separate libtorch ops of RoPE::apply_rotary_pos_emb do, rope.rs:206-248).  Element qf[8*i + e] is
@@ -333,8 +364,11 @@ __device__ __forceinline__ uint32_t fp8x2_to_f16x2(uint32_t t) {
     return (t & 0x80008000u) | ((t >> 1) & 0x3f803f80u);
 }
 
-template <int kD, bool FP8, bool ROPE, bool BAL>
+// kMode 0: every cached token, 1: sliding window with sinks, 2: as 1 (the window may be off) and the scores go to
+// a.logits, from which decode_weights_kernel makes the softmax weights once the row statistics are known.
+template <int kD, bool FP8, bool ROPE, bool BAL, int kMode = 0>
 __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
+    static_assert(kMode == 0 || !BAL, "windows and weights run on fixed chunks");
     const DecodeArgs &a = a_in;
     constexpr int kStep = Shape<kD>::kStep, NT = Shape<kD>::NT, NJ = Shape<kD>::NJ, NC = Shape<kD>::NC;
     constexpr int VW = Shape<kD>::VW, NBB = Shape<kD>::NBB, CW = Shape<kD>::CW, NS = Shape<kD>::NS;
@@ -348,9 +382,15 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
     __shared__ __attribute__((aligned(16))) float sm_sc[kWavesPerWg][64 * NS];
     __shared__ float sm_m[kWavesPerWg][16], sm_l[kWavesPerWg][16];
     __shared__ float sm_o[kWavesPerWg][16][CW + 4];  // one column group of O at a time
-    // One work item: tokens [t_begin, t_end) of sequence b (L cached tokens), partial slot `chunk`.
+    // One work item: tokens [t_begin, t_end) of sequence b (L cached tokens), partial slot `chunk`.  (kMode >= 1: t_begin
+    // and t_end count on the visible line, `line`.)
     struct Item {
         int b, L, t_begin, t_end, chunk;
+    };
+    VisibleLine line = {0, 0, 0, 0};
+    auto actual = [&](int t0) {  // first token of the step that starts at t0 on the line
+        if constexpr (kMode == 0) return t0;
+        else return t0 < line.cut ? t0 : t0 + line.skip;
     };
     // The two stages of the load pipeline and the location of the step this wavefront loads next live outside an
     // item: a workgroup that walks several items (balanced mode) issues the first loads of the next item before it
@@ -374,7 +414,7 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
     // wavefront 0, V by wavefront 1).  With five or more steps the token sits beyond every wavefront's first tile,
     // so those first loads are issued ahead of the write and its barrier instead of behind them.
     const int t_begin = it.t_begin, t_end = it.t_end;
-    const bool writes_new = a.nt.src[0] != nullptr && t_end == L;
+    const bool writes_new = a.nt.src[0] != nullptr && t_end == (kMode == 0 ? L : line.len);
     auto write_new_token = [&]() {
         if (wave < 2) quantize_row<kD / 64, FP8>(a.nt, wave, (int64_t)b * a.Hkv + h, lane);
         __syncthreads();  // codes and scales are visible to the whole workgroup before any load that covers them
@@ -398,12 +438,12 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
     auto locate = [&](const Item &w, int step) {
         const int t0 = w.t_begin + step * kStep;
         if (t0 < w.t_end) {
-            resolve(a.ka, w.b, t0, nku, nks);
-            resolve(a.va, w.b, t0, nvu, nvs);
+            resolve(a.ka, w.b, actual(t0), nku, nks);
+            resolve(a.va, w.b, actual(t0), nvu, nvs);
         }
     };
     auto load_stage = [&](Stage<kD> &st, const Item &w, int step) {
-        const int t0 = w.t_begin + step * kStep;
+        const int t0 = actual(w.t_begin + step * kStep);
         const int64_t ku = nku, vu = nvu;
         const int kslot = nks, vslot = nvs;
         locate(w, step + kWavesPerWg);
@@ -442,7 +482,7 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
     };
 
     auto compute_stage = [&](const Stage<kD> &st, int step) {
-        const int t0 = t_begin + step * kStep;
+        const int t0 = actual(t_begin + step * kStep);
         // ---- token scales: lane (li, lq) needs those of tokens 16u + 4*lq + r, the rows of its score registers.
         //      LDS operations of one wavefront complete in order, so the reads see the write without a barrier.
         float4v sk[NT], sv[NT];
@@ -476,6 +516,9 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
                                   __builtin_amdgcn_perm(0x64646464u, x0, 0x04030402u),
                                   __builtin_amdgcn_perm(0x64646464u, x1, 0x04010400u),
                                   __builtin_amdgcn_perm(0x64646464u, x1, 0x04030402u));
+                    // the weights are an fp32 output: the offset comes off exactly here instead of through the
+                    // accumulator, where it costs five bits of the score (1152 against codes of about 40)
+                    if constexpr (kMode == 2) ak -= (_Float16)1152.0f;
                 }
                 s[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ak, qop[j], s[u], 0, 0, 0);
             }
@@ -499,6 +542,27 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
                         sc[4 * u + r] = -INFINITY;
                         pv[4 * u + r] = 0.0f;
                     }
+        }
+        if constexpr (kMode >= 1) {
+            if (t0 < line.wbegin) {  // a step at the end of the sinks or at the start of the window
+#pragma unroll
+                for (int u = 0; u < NT; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int t = t0 + 16 * u + 4 * lq + r;
+                        if (t >= a.sinks && t < line.wbegin) {
+                            sc[4 * u + r] = -INFINITY;
+                            pv[4 * u + r] = 0.0f;
+                        }
+                    }
+            }
+        }
+        if constexpr (kMode == 2) {
+            if (li < G) {
+                float *row = a.logits + ((int64_t)b * a.Hq + h * G + li) * a.logit_stride + t_begin + step * kStep + 4 * lq;
+#pragma unroll
+                for (int u = 0; u < NT; ++u) *(float4v *)(row + 16 * u) = (float4v){sc[4 * u], sc[4 * u + 1], sc[4 * u + 2], sc[4 * u + 3]};
+            }
         }
         // ---- online softmax (max shared by the 4 lanes of a head)
         float mx = sc[0];
@@ -618,7 +682,7 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
             cq = a.scale_log2e * up;
             if (FP8) {
                 cq *= 256.0f * a.ks[(int64_t)b * a.Hkv + h];  // 2^8 rebias of the fp16 view of e4m3
-            } else {
+            } else if (kMode < 2) {
                 cinit = -1152.0f * qsum;
             }
         }
@@ -687,7 +751,7 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
             }
         }
     }
-    if (!a.direct && threadIdx.x < G) {
+    if ((kMode == 2 || !a.direct) && threadIdx.x < G) {
         const int g = threadIdx.x;
         float Mg = sm_m[0][g];
         for (int w = 1; w < kWavesPerWg; ++w) Mg = fmaxf(Mg, sm_m[w][g]);
@@ -712,12 +776,17 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
         const int slot = (int)((blockIdx.x + blockIdx.y + blockIdx.z) % gridDim.x);
         const int L = min(a.seq_lens[b], a.max_seq_len);
         const int t_begin = slot * a.chunk_tokens;
-        if (t_begin >= L) {
+        int len = L;
+        if constexpr (kMode >= 1) {
+            line = visible_line(L, a.window, a.sinks, kStep);
+            len = line.len;
+        }
+        if (t_begin >= len) {
             if (slot == 0 && a.direct)  // a sequence without cached tokens: its output rows are zero
                 for (int i = threadIdx.x; i < G * kD; i += 256) a.out[((int64_t)b * a.Hq + h * G) * kD + i] = 0;
             return;
         }
-        const Item it = {b, L, t_begin, min(L, t_begin + a.chunk_tokens), slot};
+        const Item it = {b, L, t_begin, min(len, t_begin + a.chunk_tokens), slot};
         run_item(it, false, it, false);
     } else {
         __shared__ int sm_pref[kMaxBalancedB + 1];  // granules before sequence b
@@ -788,9 +857,9 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
 __global__ __launch_bounds__(256) void decode_merge_kernel(const float *part_o, const float *part_ml,
                                                           const int32_t *seq_lens, uint16_t *out, const uint16_t *out_gate, int Hq, int nchunks,
                                                           int chunk_tokens, int max_seq_len, int kD, int B, int pieces,
-                                                          int min_granules) {
+                                                          int min_granules, int window, int sinks) {
     const int hq = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-    const int L = min(seq_lens[b], max_seq_len);
+    const int L = visible_line(min(seq_lens[b], max_seq_len), window, sinks, 4096 / kD).len;
     __shared__ float sm_max[4], sm_l[16];
     __shared__ __attribute__((aligned(16))) float sm_o[1024];
     __shared__ int sm_cnt[2][4];
@@ -855,6 +924,59 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(const float *part_o, 
     }
 }
 
+// The softmax weights of one decode step added up over the query heads of each kv-head (kMode 2 above):
+//   out[b, h, t] = in[b, h, t] + sum_g exp2(logit[b, hG + g, t] - m_g) / l_g,   t < L
+// with m_g and l_g joined from the chunk partials.  Grid (token blocks of 1024, kv-heads, sequences), four tokens per
+// thread.  Tokens outside the window keep their value.
+__global__ __launch_bounds__(256) void decode_weights_kernel(const float *logits, int64_t logit_stride, const float *part_ml,
+                                                            const int32_t *seq_lens, const float *in, float *out,
+                                                            int64_t stride, int Hq, int G, int nchunks, int chunk_tokens,
+                                                            int max_seq_len, int window, int sinks, int step) {
+    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
+    const int L = min(seq_lens[b], max_seq_len);
+    const int t0 = blockIdx.x * 1024;
+    if (t0 >= L) return;
+    const VisibleLine line = visible_line(L, window, sinks, step);
+    const int n = min(nchunks, (line.len + chunk_tokens - 1) / chunk_tokens);
+    __shared__ float sm_m[16], sm_inv[16];
+    for (int g = tid >> 6; g < G; g += 4) {
+        const float *ml = part_ml + ((int64_t)b * Hq + h * G + g) * nchunks * 2;
+        float m = -INFINITY, l = 0.0f;
+        for (int c = lane; c < n; c += 64) m = fmaxf(m, ml[2 * c]);
+        m = wave_max(m);
+        for (int c = lane; c < n; c += 64) l += ml[2 * c + 1] * __builtin_amdgcn_exp2f(ml[2 * c] - m);
+        l = wave_sum(l);
+        if (lane == 0) {
+            sm_m[g] = m;
+            sm_inv[g] = 1.0f / l;
+        }
+    }
+    __syncthreads();
+    const int t = t0 + 4 * tid;
+    if (t >= L) return;
+    const int64_t o = ((int64_t)b * gridDim.y + h) * stride + t;
+    const float *row = logits + ((int64_t)b * Hq + h * G) * logit_stride;
+    const bool hidden = t >= line.cut && t < line.cut + line.skip;  // (cut and skip are multiples of four)
+    if (hidden && in == out) return;
+    float4v w = in != nullptr ? *(const float4v *)(in + o) : (float4v){0.f, 0.f, 0.f, 0.f};
+    if (!hidden) {
+        const int tv = t < line.cut ? t : t - line.skip;
+        float4v add = {0.f, 0.f, 0.f, 0.f};
+        for (int g = 0; g < G; ++g) {
+            const float4v s = *(const float4v *)(row + g * logit_stride + tv);
+            const float m = sm_m[g], inv = sm_inv[g];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) add[e] += __builtin_amdgcn_exp2f(s[e] - m) * inv;
+        }
+        w += add;
+    }
+    if (t + 4 <= L) {
+        *(float4v *)(out + o) = w;
+    } else {
+        for (int e = 0; e < L - t; ++e) out[o + e] = w[e];
+    }
+}
+
 // The balanced instances read their arguments anew from the kernel-argument segment, reinterpreted as DecodeArgs:
 // that is only right while DecodeArgs is the kernel's sole parameter (it then starts at offset 0 of the segment) and
 // is passed by value as plain bytes.
@@ -866,6 +988,16 @@ int validate_layout(const hs_kv_layout *l, int B, int S, int Hkv, int D, bool ne
 int check_prologue(const hs_qk_prologue *p, int dtype, int D, bool need_q, bool need_k);
 NormSpec norm_spec(const hs_qk_prologue *p, int which);
 
+// Rows of accumulated weights [B, Hkv, stride] fp32, read and written 16 bytes at a time.
+int check_weights(const float *in, const float *out, int64_t stride, int max_seq_len, bool used) {
+    if (used && !out) return fail(HS_ERR_INVALID_ARGUMENT, "null weights");
+    if ((((uintptr_t)in | (uintptr_t)out) & 15) != 0 || (stride & 3) != 0)
+        return fail(HS_ERR_INVALID_ARGUMENT, "weights must be 16-byte aligned, with a stride that is a multiple of 4");
+    if (stride < max_seq_len)
+        return fail(HS_ERR_OVERFLOW, "weights_stride %lld is below max_seq_len %d", (long long)stride, max_seq_len);
+    return HS_OK;
+}
+
 // Workgroups of a balanced launch: two resident on each of 256 CUs, one round.  Measured at B=64, lengths U[512, 8192]
 // (us per step): 116 with 512, 139 with 640 and 768, 125 with 1024, 129 with 1536, 136 with 2048 -- a second, partial
 // round costs more than the finer balance gains.
@@ -876,6 +1008,7 @@ struct Split {
     int balanced, pieces, min_granules;   // balanced token ranges: grid (pieces, Hkv), nchunks = partial slots per sequence
 };
 
+// (max_seq_len: tokens that count, i.e. the longest visible line of a windowed call, which then gives no hint.)
 static Split pick_split(int B, int Hkv, int max_seq_len, int64_t total_tokens_hint) {
     Split s{};
     // A workgroup costs about 1.5 us of prologue/epilogue, so chunks are as long as the grid allows:
@@ -935,12 +1068,20 @@ struct NewToken {  // optional quantize-on-write of one token per sequence insid
     bool prologue = false;                                // the kernel instance with the q-side prologue
 };
 
+struct WeightsOut {  // optional: softmax weights of the step, summed over the heads of a group and added to `in`
+    const float *in = nullptr;
+    float *out = nullptr;
+    int64_t stride = 0;  // elements between kv-heads; sequences are Hkv * stride apart
+};
+
+static int64_t logit_row(int tokens) { return ((int64_t)tokens + 63) / 64 * 64; }
+
 // static_scratch: the partials go to this device's copy of `scratch` (ws / ws_bytes ignored) and the size check is
 // against what THIS call's split needs, not the worst case a caller-sized workspace has to cover.
 static int launch_decode(bool fp8, int phases, const NewToken &nt, const void *q, void *kc, void *vc, float *ks,
                          float *vs, const hs_kv_layout *l, const int32_t *seq_lens, void *out, void *ws,
                          size_t ws_bytes, int B, int Hq, int Hkv, int D, int max_seq_len, float softmax_scale,
-                         hipStream_t stream, bool static_scratch = false) {
+                         hipStream_t stream, bool static_scratch = false, const WeightsOut &wt = WeightsOut()) {
     if (int rc = validate_layout(l, B, 0, Hkv, D, !fp8)) return rc;
     if (D != 64 && D != 128 && D != 256)
         return fail(HS_ERR_INVALID_ARGUMENT, "decode attention is built for head_dim 64, 128 and 256, got %d", D);
@@ -951,6 +1092,8 @@ static int launch_decode(bool fp8, int phases, const NewToken &nt, const void *q
     if (Hq <= 0 || Hq % Hkv != 0 || Hq / Hkv > 16)
         return fail(HS_ERR_INVALID_ARGUMENT, "need Hq %% Hkv == 0 and Hq/Hkv <= 16 (Hq=%d Hkv=%d)", Hq, Hkv);
     if (max_seq_len <= 0) return fail(HS_ERR_INVALID_ARGUMENT, "max_seq_len must be positive");
+    if (l->decode_window < 0 || l->attn_sinks < 0)
+        return fail(HS_ERR_INVALID_ARGUMENT, "negative decode_window %d or attn_sinks %d", l->decode_window, l->attn_sinks);
     if (l->k_block_table && (l->capacity_tokens % (D == 64 ? 64 : 32)) != 0)  // a wavefront step stays inside one block
         return fail(HS_ERR_INVALID_ARGUMENT, "paged blocks must hold a multiple of %d tokens", D == 64 ? 64 : 32);
     if (B == 0) return HS_OK;
@@ -961,7 +1104,15 @@ static int launch_decode(bool fp8, int phases, const NewToken &nt, const void *q
                         (long long)cap);
     }
     DecodeArgs a;
-    const Split sp = pick_split(B, Hkv, max_seq_len, l->total_tokens_hint);
+    const bool weights = wt.out != nullptr;
+    const int step = 4096 / D;
+    a.window = l->decode_window;
+    a.sinks = l->attn_sinks;
+    const int mode = weights ? 2 : a.window > 0 ? 1 : 0;
+    // Windowed sequences are nearly all of one length on the visible line, and the scores of a step live in rows of a
+    // fixed length: both keep fixed chunks whatever the hint says.
+    const int line = visible_bound(max_seq_len, a.window, a.sinks, step);
+    const Split sp = pick_split(B, Hkv, line, mode != 0 ? 0 : l->total_tokens_hint);
     a.chunk_tokens = sp.chunk_tokens; a.nchunks = sp.nchunks;
     a.balanced = sp.balanced; a.pieces = sp.pieces; a.min_granules = sp.min_granules;
     if (static_scratch) {
@@ -974,7 +1125,8 @@ static int launch_decode(bool fp8, int phases, const NewToken &nt, const void *q
         if (need > 0)
             if (int rc = claim_scratch(stream)) return rc;
     } else {
-        const size_t need = hs_decode_attn_workspace_bytes(B, Hq, Hkv, D, max_seq_len);
+        const size_t need = weights ? hs_decode_weights_workspace_bytes(B, Hq, Hkv, D, max_seq_len)
+                                    : hs_decode_attn_workspace_bytes(B, Hq, Hkv, D, max_seq_len);
         if (!ws || ws_bytes < need)
             return fail(HS_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed", ws_bytes, need);
         if (((uintptr_t)ws & 255) != 0) return fail(HS_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
@@ -985,6 +1137,13 @@ static int launch_decode(bool fp8, int phases, const NewToken &nt, const void *q
     a.ka = make_addr(*l, 0); a.va = make_addr(*l, 1);
     a.seq_lens = seq_lens;
     a.B = B; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv; a.max_seq_len = max_seq_len;
+    a.logits = nullptr;
+    a.logit_stride = 0;
+    if (weights) {
+        a.logits = (float *)ws;
+        a.logit_stride = logit_row(line);
+        ws = a.logits + (size_t)B * Hq * a.logit_stride;
+    }
     a.part_o = (float *)ws;
     a.part_ml = a.part_o + (size_t)B * Hq * a.nchunks * D;
     a.out = (uint16_t *)out;
@@ -1022,21 +1181,32 @@ static int launch_decode(bool fp8, int phases, const NewToken &nt, const void *q
                         "hs_qk_prologue_apply (which takes any alignment) and hs_decode_step_* instead");
     if (phases & 1) {
         const dim3 grid = a.balanced ? dim3(a.pieces, Hkv, 1) : dim3(a.nchunks, Hkv, B);
-#define HS_DECODE_LAUNCH(DD, BAL)                                                                      \
+#define HS_DECODE_LAUNCH(DD, ...)  /* head_dim, balanced[, mode] */                                    \
     do {                                                                                               \
-        if (fp8 && pro) decode_attn_kernel<DD, true, true, BAL><<<grid, 256, 0, stream>>>(a);          \
-        else if (fp8) decode_attn_kernel<DD, true, false, BAL><<<grid, 256, 0, stream>>>(a);           \
-        else if (pro) decode_attn_kernel<DD, false, true, BAL><<<grid, 256, 0, stream>>>(a);           \
-        else decode_attn_kernel<DD, false, false, BAL><<<grid, 256, 0, stream>>>(a);                   \
+        if (fp8 && pro) decode_attn_kernel<DD, true, true, __VA_ARGS__><<<grid, 256, 0, stream>>>(a);  \
+        else if (fp8) decode_attn_kernel<DD, true, false, __VA_ARGS__><<<grid, 256, 0, stream>>>(a);   \
+        else if (pro) decode_attn_kernel<DD, false, true, __VA_ARGS__><<<grid, 256, 0, stream>>>(a);   \
+        else decode_attn_kernel<DD, false, false, __VA_ARGS__><<<grid, 256, 0, stream>>>(a);           \
     } while (0)
         if (a.balanced) {
             if (D == 64) HS_DECODE_LAUNCH(64, true);
             else if (D == 128) HS_DECODE_LAUNCH(128, true);
             else HS_DECODE_LAUNCH(256, true);
-        } else {
+        } else if (mode == 0) {
             if (D == 64) HS_DECODE_LAUNCH(64, false);
             else if (D == 128) HS_DECODE_LAUNCH(128, false);
             else HS_DECODE_LAUNCH(256, false);
+        } else if (mode == 1) {
+            if (D == 64) HS_DECODE_LAUNCH(64, false, 1);
+            else if (D == 128) HS_DECODE_LAUNCH(128, false, 1);
+            else HS_DECODE_LAUNCH(256, false, 1);
+        } else {  // (the entry point that asks for weights takes no prologue)
+            if (D == 64 && fp8) decode_attn_kernel<64, true, false, false, 2><<<grid, 256, 0, stream>>>(a);
+            else if (D == 64) decode_attn_kernel<64, false, false, false, 2><<<grid, 256, 0, stream>>>(a);
+            else if (D == 128 && fp8) decode_attn_kernel<128, true, false, false, 2><<<grid, 256, 0, stream>>>(a);
+            else if (D == 128) decode_attn_kernel<128, false, false, false, 2><<<grid, 256, 0, stream>>>(a);
+            else if (fp8) decode_attn_kernel<256, true, false, false, 2><<<grid, 256, 0, stream>>>(a);
+            else decode_attn_kernel<256, false, false, false, 2><<<grid, 256, 0, stream>>>(a);
         }
 #undef HS_DECODE_LAUNCH
         if (int rc = check_launch("decode_attn")) return rc;
@@ -1044,8 +1214,14 @@ static int launch_decode(bool fp8, int phases, const NewToken &nt, const void *q
     if ((phases & 2) && !a.direct) {
         decode_merge_kernel<<<dim3(Hq, B), 256, 0, stream>>>(a.part_o, a.part_ml, seq_lens, (uint16_t *)out, a.out_gate, Hq,
                                                                a.nchunks, a.chunk_tokens, max_seq_len, D, B,
-                                                               a.balanced ? a.pieces : 0, a.min_granules);
-        return check_launch("decode_merge");
+                                                               a.balanced ? a.pieces : 0, a.min_granules, a.window, a.sinks);
+        if (int rc = check_launch("decode_merge")) return rc;
+    }
+    if (weights) {
+        decode_weights_kernel<<<dim3((max_seq_len + 1023) / 1024, Hkv, B), 256, 0, stream>>>(
+            a.logits, a.logit_stride, a.part_ml, seq_lens, wt.in, wt.out, wt.stride, Hq, a.G, a.nchunks, a.chunk_tokens,
+            max_seq_len, a.window, a.sinks, step);
+        return check_launch("decode_weights");
     }
     return HS_OK;
 }
@@ -1164,6 +1340,26 @@ int hs_decode_step_fp8(const void *q, const void *k_new, const void *v_new, int 
     return hs::launch_decode(true, 3, nt, q, k_codes, v_codes, (float *)k_scales, (float *)v_scales, layout, seq_lens,
                              out, workspace, workspace_bytes, B, Hq, Hkv, D, max_seq_len, softmax_scale,
                              (hipStream_t)stream);
+}
+
+size_t hs_decode_weights_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_seq_len) {
+    if (B <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0 || max_seq_len <= 0) return 0;
+    // the scores' rows (of the longest visible line any window leaves: all tokens), then the partials
+    return (size_t)B * Hq * hs::logit_row(max_seq_len) * sizeof(float) + hs_decode_attn_workspace_bytes(B, Hq, Hkv, D, max_seq_len);
+}
+
+int hs_decode_step_weights(int fmt_fp8, const void *q, const void *k_new, const void *v_new, int src_dtype, void *k_codes,
+                           void *v_codes, float *k_scales, float *v_scales, const hs_kv_layout *layout,
+                           const int32_t *seq_lens, void *out, const float *weights_in, float *weights_out,
+                           int64_t weights_stride, void *workspace, size_t workspace_bytes, int32_t B, int32_t Hq,
+                           int32_t Hkv, int32_t D, int32_t max_seq_len, float softmax_scale, hs_stream_t stream) {
+    if (int rc = hs::check_weights(weights_in, weights_out, weights_stride, max_seq_len, B > 0)) return rc;
+    hs::NewToken nt;
+    nt.k_src = k_new; nt.v_src = v_new; nt.dtype = src_dtype;
+    hs::WeightsOut wt;
+    wt.in = weights_in; wt.out = weights_out; wt.stride = weights_stride;
+    return hs::launch_decode(fmt_fp8 != 0, 3, nt, q, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, workspace,
+                             workspace_bytes, B, Hq, Hkv, D, max_seq_len, softmax_scale, (hipStream_t)stream, false, wt);
 }
 
 int hs_decode_attn_phases(int fmt_fp8, int phases, const void *q, const void *k_codes, const void *v_codes,

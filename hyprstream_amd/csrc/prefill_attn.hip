@@ -155,7 +155,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
     const bool wv_active = wv_q0 < S;
     // Sliding window: the query in-call index i sees the keys whose distance to it is below W.  The first visible key
     // of the workgroup's (wavefront's) first query bounds where the walks start; steps below a wavefront's bound are
-    // skipped by that wavefront, steps that a bound cuts through take the masking path of the softmax.
+    // skipped by that wavefront, steps that a bound cuts through take the masking path of the softmax.  The first a.sinks
+    // tokens of the sequence stay visible: their steps (in the history, or in the call's own tokens where the history is
+    // shorter than they are) come ahead of both walks.
     const int W = kWin && a.window > 0 ? a.window : (1 << 30);
     // in-call index of the first key column nb sees (negative: that many history tokens back)
     auto qlo = [&](int nb) { return min(qi[nb], S - 1) - W + 1; };
@@ -323,6 +325,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
         constexpr int kHStep = 64;
         const int nsteps = kSplit ? h_hi : (H + kHStep - 1) / kHStep;
         const int st0 = kSplit ? h_lo : kWin ? min(max(H + wg_lo, 0) / kHStep, nsteps) : 0;  // first step that holds a key some query of the workgroup sees
+        // the sinks' steps ahead of it: the walk takes those, then goes on at st0
+        const int sink_steps = kWin ? min((min(a.sinks, H) + kHStep - 1) / kHStep, st0) : 0;
+        auto step_from = [&](int st) { return kWin && st >= sink_steps && st < st0 ? st0 : st; };
         HistTile *htiles = (HistTile *)lds;
         // ---- producers: every wavefront converts one eighth of the step's K tiles and of its V tiles.
         //      K: wavefront w takes 16-key block u4 = w/2 and the d-halves jp = w%2 of every 32-d group: lane
@@ -366,6 +371,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
         auto issue = [&](int step) {
             const int t0 = step * kHStep;
             const int last = H - 1 - t0;
+            if (kWin && step == st0) kleft = vleft = 0;  // behind the sinks the cursors start anew
             if (kleft <= 0) {
                 int64_t unit;
                 int slot;
@@ -549,11 +555,12 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
                         }
                         if (edge) {
                             const int first = H + qlo(nb) - step * kHStep - 4 * lq;  // key offsets 16u4 + r below this are out of the window
+                            const int sink_end = a.sinks - step * kHStep - 4 * lq;   // unless they are below this
 #pragma unroll
                             for (int u4 = 0; u4 < 4; ++u4)
 #pragma unroll
                                 for (int r = 0; r < 4; ++r)
-                                    if (16 * u4 + r < first) e[nb][4 * u4 + r] = -INFINITY;
+                                    if (16 * u4 + r < first && 16 * u4 + r >= sink_end) e[nb][4 * u4 + r] = -INFINITY;
                         }
                         float m = e[nb][0];
 #pragma unroll
@@ -628,18 +635,23 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
             }
         };
         auto walk = [&](auto softmax) {
-            if (st0 >= nsteps) return;  // the window of every query of the workgroup starts after the history
-            issue(st0);
-            commit(htiles[st0 & 1], st0);
-            if (st0 + 1 < nsteps) issue(st0 + 1);
+            const int begin = kSplit ? st0 : step_from(0);
+            if (begin >= nsteps) return;  // the window of every query of the workgroup starts after the history
+            const int second = step_from(begin + 1);
+            issue(begin);
+            commit(htiles[begin & 1], begin);
+            if (second < nsteps) issue(second);
             lds_barrier();
-            for (int st = st0; st < nsteps; ++st) {
+            int next = second, buf = begin & 1;
+            for (int st = begin; st < nsteps; st = next, buf ^= 1) {
+                next = step_from(st + 1);
+                const int after = step_from(next + 1);
                 if (!late) {
-                    if (st + 1 < nsteps) commit(htiles[(st + 1) & 1], st + 1);
-                    if (st + 2 < nsteps) issue(st + 2);
+                    if (next < nsteps) commit(htiles[buf ^ 1], next);
+                    if (after < nsteps) issue(after);
                 }
-                const HistTile &t = htiles[st & 1];
-                if (!kWin || st * kHStep + kHStep > H + wv_lo) {  // else: no query of this wavefront sees a key of the step
+                const HistTile &t = htiles[buf];
+                if (!kWin || st * kHStep + kHStep > H + wv_lo || st * kHStep < a.sinks) {  // else: no query of this wavefront sees a key of the step
                     if constexpr (kRing) {
                         scores_ahead(t);
                         softmax(st);
@@ -654,8 +666,8 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
                     }
                 }
                 if (late) {
-                    if (st + 1 < nsteps) commit(htiles[(st + 1) & 1], st + 1);
-                    if (st + 2 < nsteps) issue(st + 2);
+                    if (next < nsteps) commit(htiles[buf ^ 1], next);
+                    if (after < nsteps) issue(after);
                 }
                 lds_barrier();
             }
@@ -703,6 +715,9 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
         constexpr int kNStep = 64;
         const int nsteps = kSplit ? n_hi : wg_qlast / kNStep + 1;
         const int st0 = kSplit ? n_lo : kWin ? max(wg_lo, 0) / kNStep : 0;  // first step with a key inside the window of the workgroup's first query
+        const int new_sinks = kWin ? max(a.sinks - H, 0) : 0;               // sinks among the call's own tokens: their steps come ahead of it
+        const int sink_steps = kWin ? min((int)(((int64_t)new_sinks + kNStep - 1) / kNStep), st0) : 0;
+        auto step_from = [&](int st) { return kWin && st >= sink_steps && st < st0 ? st0 : st; };
         HistTile *ntiles = (HistTile *)lds;
         const uint16_t *knb = a.kn + ((int64_t)b * S * a.Hkv + kvh) * kRow;
         const uint16_t *vnb = a.vn + ((int64_t)b * S * a.Hkv + kvh) * kRow;
@@ -769,7 +784,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
         bf16x8 pop[kNB][2];
         // Halves of step `step` that hold a key some query of this wavefront may see (0: the step is skipped).
         auto halves = [&](int step) {
-            if (!wv_active || step * kNStep > wv_qlast || (kWin && step * kNStep + kNStep <= wv_lo)) return 0;
+            if (!wv_active || step * kNStep > wv_qlast || (kWin && step * kNStep + kNStep <= wv_lo && step * kNStep >= new_sinks)) return 0;
             return step * kNStep + 32 > wv_qlast ? 1 : 2;
         };
         constexpr int KU = kPD == 128 && kWaves == 8 ? 2 : 1;  // 16-key tiles whose K operands are read at once
@@ -849,7 +864,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
                     for (int u4 = 0; u4 < 4; ++u4)
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
-                            if (16 * u4 + r > qrel || (kWin && 16 * u4 + r < qrel - W + 1)) e[nb][4 * u4 + r] = -INFINITY;
+                            if (16 * u4 + r > qrel || (kWin && 16 * u4 + r < qrel - W + 1 && 16 * u4 + r >= new_sinks - t0 - 4 * lq)) e[nb][4 * u4 + r] = -INFINITY;
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) over = max(over, __float_as_int(e[nb][i]));
@@ -956,16 +971,20 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
             }
         }
         if (new_here) {
-        issue(st0);
-        commit(ntiles[st0 & 1]);
-        if (st0 + 1 < nsteps) issue(st0 + 1);
+        const int begin = kSplit ? st0 : step_from(0);
+        int next = step_from(begin + 1), buf = begin & 1;
+        issue(begin);
+        commit(ntiles[buf]);
+        if (next < nsteps) issue(next);
         lds_barrier();
-        for (int st = st0; st < nsteps; ++st) {
-            if (st + 1 < nsteps) commit(ntiles[(st + 1) & 1]);
-            if (st + 2 < nsteps) issue(st + 2);
+        for (int st = begin; st < nsteps; st = next, buf ^= 1) {
+            next = step_from(st + 1);
+            const int after = step_from(next + 1);
+            if (next < nsteps) commit(ntiles[buf ^ 1]);
+            if (after < nsteps) issue(after);
             const int nh = halves(st);
             if (nh > 0) {
-                const HistTile &t = ntiles[st & 1];
+                const HistTile &t = ntiles[buf];
                 scores(t, nh);
                 load_v(t, 0);
                 softmax(st, nh, std::integral_constant<int, 0>{});
@@ -1127,7 +1146,8 @@ static int launch_prefill(bool fp8, const void *q, const void *k_new, const void
     if ((hist_len > 0 || quantize_on_write) && (!k_codes || !v_codes || !k_scales || !v_scales))
         return fail(HS_ERR_INVALID_ARGUMENT, "null cache buffer");
     if (hist_len < 0) return fail(HS_ERR_INVALID_ARGUMENT, "negative hist_len");
-    if (layout->prefill_window < 0) return fail(HS_ERR_INVALID_ARGUMENT, "negative prefill_window");
+    if (layout->prefill_window < 0 || layout->attn_sinks < 0)
+        return fail(HS_ERR_INVALID_ARGUMENT, "negative prefill_window or attn_sinks");
     const int G = Hq > 0 && Hkv > 0 ? Hq / Hkv : 0;
     if (Hq <= 0 || Hq % Hkv != 0)
         return fail(HS_ERR_INVALID_ARGUMENT, "need Hq %% Hkv == 0 (Hq=%d Hkv=%d)", Hq, Hkv);
@@ -1151,6 +1171,7 @@ static int launch_prefill(bool fp8, const void *q, const void *k_new, const void
     a.hist_lens = hist_lens;
     a.write_new = quantize_on_write ? 1 : 0;
     a.window = layout->prefill_window;
+    a.sinks = layout->attn_sinks;
     if (const hs_qk_prologue *qp = layout->prefill_q_prologue) {
         if (int rc = check_prologue(qp, HS_BF16, D, true, false)) return rc;
         const int rd = qp->rotary_dim > 0 ? qp->rotary_dim : D;

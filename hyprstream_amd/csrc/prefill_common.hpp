@@ -28,6 +28,7 @@ struct PrefillArgs {
     int32_t heavy_first;  // the grid outnumbers the CUs: order the query tiles by decreasing work
     int32_t write_new;    // quantize-on-write of the call's K/V rows by the workgroups that finish early
     int32_t window;       // sliding window of local layers: a query at position p attends keys in (p - window, p]; 0 = none
+    int32_t sinks;        // with a window: the first tokens of the sequence that stay visible
     float scale_log2e;
     // keys of a query tile split over nsplit workgroups (prefill_attn_kernel<..., kSplit>): partial accumulators and an
     // arrival counter per tile in the caller's workspace; the workgroup that arrives last merges and stores

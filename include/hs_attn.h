@@ -94,7 +94,8 @@ typedef struct hs_kv_layout {
                                    position p attends the keys in (p - window, p].  0 = no window.  For a prompt on an
                                    empty cache this is the reference's mask; with history it is the same rule on
                                    absolute positions (the reference's [q_len, q_len] mask has no meaning there).
-                                   Decode entry points ignore it, as the reference applies no window at q_len == 1. */
+                                   Decode entry points ignore it, as the reference applies no window at q_len == 1;
+                                   decode_window below is theirs. */
     const void *out_gate;       /* attention calls, optional: bf16, device, the shape of `out`.  The output gate of the
                                    Qwen3.5 full-attention layers (qwen3_5.rs:1056-1059: ctx * sigmoid(gate) in the model
                                    dtype): out = bf16(bf16(attention) * bf16(sigmoid(gate))) written by the same launch.
@@ -110,7 +111,10 @@ typedef struct hs_kv_layout {
     void *prefill_split_workspace;
     int64_t prefill_split_workspace_bytes;
     int32_t prefill_key_splits;
-    int32_t reserved0;          /* prefill only, optional: device scratch that lets a call whose query tiles are too few
+    int32_t attn_sinks;         /* with a window (prefill_window, decode_window), optional: the first attn_sinks tokens of
+                                   a sequence stay visible whatever the window has left behind.  0 = none; without a
+                                   window it changes nothing. */
+                                /* prefill_split_workspace, prefill_key_splits: prefill only, optional: device scratch that lets a call whose query tiles are too few
                                    to occupy the GPU (a chunk of ONE sequence: 64 tiles on 256 compute units) cut the
                                    keys of every tile into runs for several workgroups, the last of which to finish
                                    merges the partial results.  At least hs_prefill_attn_split_workspace_bytes(...)
@@ -128,7 +132,13 @@ typedef struct hs_kv_layout {
     void *prefill_shadow;
     int64_t prefill_shadow_bytes;
     int32_t prefill_shadow_tokens;
-    int32_t reserved1;          /* prefill only, optional, head_dim 128 (int8 or fp8 cache): a bf16 copy of the prompt's
+    int32_t decode_window;      /* decode only, optional: the newest token, at position p = seq_lens[b] - 1, attends the
+                                   keys in (p - decode_window, p] and the first attn_sinks tokens.  0 = every cached
+                                   token.  Only the visible tokens are read, so a step costs what the window holds
+                                   however long the sequence is.  Served by every decode entry point; the chunks then
+                                   follow the window's length (hs_decode_attn_num_chunks answers for calls without one)
+                                   and total_tokens_hint is not used.  The workspace for max_seq_len covers it. */
+                                /* prefill_shadow: prefill only, optional, head_dim 128 (int8 or fp8 cache): a bf16 copy of the prompt's
                                    DEQUANTIZED K/V (code * scale, the values the reference's get() hands to its
                                    attention, kv_cache.rs:1493-1560) in the order the matrix instructions take them,
                                    kept by the caller for as long as one prompt is being prefilled into one layer's
@@ -355,6 +365,71 @@ HS_API int hs_decode_attn_phases(int fmt_fp8, int phases, const void *q, const v
                                  const int32_t *seq_lens, void *out, void *workspace, size_t workspace_bytes,
                                  int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_seq_len,
                                  float softmax_scale, hs_stream_t stream);
+
+/* ---- what a bounded cache needs beside the window: how much attention each cached token gets, and leaving out the
+ * tokens that get little.  No counterpart in the reference, whose caches only grow or are truncated
+ * (kv_cache.rs:1646-1735); hs_kv_evict takes the place of the overflow error there (kv_cache.rs:1288-1294). ---------
+ * Weights are fp32 rows [B, Hkv, weights_stride], one entry per cached token: entry t of row (b, h) holds the softmax
+ * weights token t has received, summed over queries and over the Hq/Hkv query heads that read kv-head h.  Rows are
+ * 16-byte aligned, weights_stride is a multiple of 4 and >= max_seq_len.  Every call computes
+ *     weights_out[b, h, t] = weights_in[b, h, t] + (the call's weights)
+ * for the tokens t below the sequence's length and leaves entries behind it as they are; weights_in NULL counts as
+ * zeros, weights_in == weights_out accumulates in place (otherwise the two may not overlap).  Sums are fp32 in a fixed
+ * order: the same call gives the same bits. */
+/* hs_decode_step_* (k_new, v_new: one new token per sequence, written at seq_lens[b] - 1 first; both NULL:
+ * hs_decode_attn_*) together with the weights of its Hq queries.  fmt_fp8 as in hs_decode_attn_phases; decode_window,
+ * attn_sinks and out_gate of the layout apply (a token the window hides receives nothing).  q and k_new arrive
+ * normalised and rotated.  Three launches at most; the workspace is hs_decode_weights_workspace_bytes(...) bytes,
+ * 256-byte aligned (the scores pass through it: 4 bytes per query head and token). */
+HS_API size_t hs_decode_weights_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_seq_len);
+HS_API int hs_decode_step_weights(int fmt_fp8, const void *q, const void *k_new, const void *v_new, int src_dtype,
+                               void *k_codes, void *v_codes, float *k_scales, float *v_scales,
+                               const hs_kv_layout *layout, const int32_t *seq_lens, void *out,
+                               const float *weights_in, float *weights_out, int64_t weights_stride,
+                               void *workspace, size_t workspace_bytes,
+                               int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_seq_len,
+                               float softmax_scale, hs_stream_t stream);
+/* The weights of S queries per sequence over keys that are all in the cache (a whole prompt after its prefill, or the
+ * last queries of one as an observation window).  q [B, S, Hq, D] bf16, normalised and rotated; query s of sequence b
+ * sits at position p = (positions ? positions[b] : 0) + start_pos + s, `positions` as for hs_kv_quantize_int8, and sees
+ * the keys t <= p (prefill_window and attn_sinks of the layout apply).  max_seq_len: host-side bound of the positions;
+ * queries whose device-side position falls outside [0, max_seq_len) contribute nothing.  The entries written are those
+ * below min(max_seq_len, last query's position + 1).  Keys are the DEQUANTIZED ones: hs_prefill_attn_* attends its own call's tokens
+ * in bf16, so its weights differ by the quantization of those keys.  D is 64, 128 or 256.  Workspace:
+ * hs_attn_weights_workspace_bytes(...) bytes, 256-byte aligned. */
+HS_API size_t hs_attn_weights_workspace_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_seq_len);
+HS_API int hs_attn_weights(int fmt_fp8, const void *q, const void *k_codes, const float *k_scales,
+                               const hs_kv_layout *layout, const int32_t *positions, int32_t start_pos,
+                               const float *weights_in, float *weights_out, int64_t weights_stride,
+                               void *workspace, size_t workspace_bytes,
+                               int32_t B, int32_t S, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_seq_len,
+                               float softmax_scale, hs_stream_t stream);
+/* Cuts every sequence of a cache down to at most `budget` tokens per kv-head and moves the ones that stay to the front,
+ * in their order.  A sequence of L = seq_lens[b] > budget tokens keeps, in every kv-head by itself, its first `sinks`
+ * tokens, its last `recent` ones and, of those between, the budget - sinks - recent with the largest weights (ties: the
+ * lower position; a NaN ranks below every number, -0 equals +0).  weights NULL: the first `sinks` and the last
+ * budget - sinks tokens.  A shorter sequence is moved whole.
+ *   *_out        where the tokens go: codes, int8 scales (fp8: the head scales are copied), by layout_out.  Either a cache
+ *                of its own (any capacity >= budget, paged or not), or the source itself: the same buffers, tables and
+ *                strides, which is done in place.  A layout_out that shares the source's buffers through other block
+ *                tables must not share blocks with it.  int8 or fp8 as the source.
+ *   seq_lens_out device [B]: min(L, budget); may be seq_lens.
+ *   weights_out  rows [B, Hkv, weights_out_stride] (alignment as above, stride >= budget): the weights of the kept tokens,
+ *                then zeros up to min(weights_out_stride, max_seq_len); NULL = not wanted; may be `weights` if the stride is the same.
+ *   kept         device [B, Hkv, budget] or NULL: old position of each token that stayed, ascending, -1 behind the last.
+ * Keys keep the rotation of the position they were written at.  After an eviction a cache holds fewer tokens than the
+ * sequence has positions: rotate new tokens by their true position (hs_qk_prologue_apply with `positions`), then cache
+ * them at seq_lens_out; the entry points that rotate by the cache position do not fit such a cache, and windows and
+ * causal masks count the tokens that are there.  max_seq_len >= every seq_lens[b].  Workspace:
+ * hs_kv_evict_workspace_bytes(...) bytes, 256-byte aligned, no initialisation. */
+HS_API size_t hs_kv_evict_workspace_bytes(int32_t B, int32_t Hkv, int32_t budget, int32_t max_seq_len);
+HS_API int hs_kv_evict(int fmt_fp8, const void *k_codes, const void *v_codes, const float *k_scales, const float *v_scales,
+                               const hs_kv_layout *layout, const int32_t *seq_lens, const float *weights, int64_t weights_stride,
+                               void *k_codes_out, void *v_codes_out, float *k_scales_out, float *v_scales_out,
+                               const hs_kv_layout *layout_out, int32_t *seq_lens_out, float *weights_out,
+                               int64_t weights_out_stride, int32_t *kept, int32_t budget, int32_t sinks, int32_t recent,
+                               void *workspace, size_t workspace_bytes,
+                               int32_t B, int32_t Hkv, int32_t D, int32_t max_seq_len, hs_stream_t stream);
 
 /* ---- causal prefill over [int8 history] + [this call's bf16 K/V] (replaces update + get +
  * compute_attention_masked for q_len > 1: llama.rs:1066-1112, mask rule "query row i sits at
