@@ -235,19 +235,32 @@ __global__ __launch_bounds__(256, 2) void weights_stats_kernel(WeightsArgs a) {
     }
 }
 
-// lse of a column from its key chunks.
+// lse of a column from its key chunks: sixteen columns a workgroup, the chunks of one over sixteen lanes.
 __global__ __launch_bounds__(256) void weights_join_kernel(WeightsArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, n = (int64_t)a.B * a.Hkv * a.cols;
-    if (i >= n) return;
-    const int64_t unit = i / a.cols, c = i % a.cols;
-    const float *ml = a.part_ml + (unit * a.key_chunks * a.cols + c) * 2;
+    const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15), n = (int64_t)a.B * a.Hkv * a.cols;
+    const int part = threadIdx.x >> 4;
+    __shared__ float sm_m[16][16], sm_l[16][16];
     float M = -INFINITY, L = 0.0f;
-    for (int k = 0; k < a.key_chunks; ++k) M = fmaxf(M, ml[(int64_t)k * a.cols * 2]);
-    for (int k = 0; k < a.key_chunks; ++k) {
-        const float m = ml[(int64_t)k * a.cols * 2], l = ml[(int64_t)k * a.cols * 2 + 1];
-        L += m == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - M);  // (a chunk without a key has l = 0; NaN stays)
+    if (i < n) {
+        const int64_t unit = i / a.cols, c = i % a.cols;
+        const float *ml = a.part_ml + (unit * a.key_chunks * a.cols + c) * 2;
+        for (int k = part; k < a.key_chunks; k += 16) M = fmaxf(M, ml[(int64_t)k * a.cols * 2]);
+        for (int k = part; k < a.key_chunks; k += 16) {
+            const float m = ml[(int64_t)k * a.cols * 2], l = ml[(int64_t)k * a.cols * 2 + 1];
+            L += m == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - M);  // (a chunk without a key has l = 0; NaN stays)
+        }
     }
-    a.lse[i] = L == 0.0f ? INFINITY : M + __builtin_amdgcn_logf(L);
+    sm_m[part][threadIdx.x & 15] = M;
+    sm_l[part][threadIdx.x & 15] = L;
+    __syncthreads();
+    if (part != 0 || i >= n) return;
+    float Mt = M, Lt = 0.0f;
+    for (int p = 1; p < 16; ++p) Mt = fmaxf(Mt, sm_m[p][threadIdx.x]);
+    for (int p = 0; p < 16; ++p) {
+        const float m = sm_m[p][threadIdx.x], l = sm_l[p][threadIdx.x];
+        Lt += m == -INFINITY ? l : l * __builtin_amdgcn_exp2f(m - Mt);
+    }
+    a.lse[i] = Lt == 0.0f ? INFINITY : Mt + __builtin_amdgcn_logf(Lt);
 }
 
 template <int D, bool FP8>
@@ -444,7 +457,7 @@ template <int D, bool FP8>
 static void launch_weights(const WeightsArgs &a, const WeightsPlan &p, hipStream_t st) {
     const int64_t units = (int64_t)a.B * a.Hkv;
     weights_stats_kernel<D, FP8><<<(unsigned)(units * p.key_chunks * p.col_blocks), 256, 0, st>>>(a);
-    if (p.key_chunks > 1) weights_join_kernel<<<(unsigned)((units * p.cols + 255) / 256), 256, 0, st>>>(a);
+    if (p.key_chunks > 1) weights_join_kernel<<<(unsigned)((units * p.cols + 15) / 16), 256, 0, st>>>(a);
     weights_columns_kernel<D, FP8><<<(unsigned)(units * p.segments * p.key_blocks), 256, 0, st>>>(a);
     if (p.segments > 1) weights_sum_kernel<<<dim3((unsigned)((a.max_seq_len + 1023) / 1024), (unsigned)units), 256, 0, st>>>(a);
 }

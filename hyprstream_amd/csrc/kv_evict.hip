@@ -15,8 +15,6 @@ namespace hs {
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
-constexpr int kSelectThreads = 1024;
-
 struct EvictArgs {
     const uint8_t *kc, *vc;
     const float *ks, *vs;
@@ -32,6 +30,7 @@ struct EvictArgs {
     int32_t *list;      // workspace [B, Hkv, budget]
     int32_t *info;      // workspace [B, Hkv, 2]: tokens kept, first list entry that moves
     int32_t budget, sinks, recent, Hkv, D, max_seq_len, fp8;
+    int32_t finish;     // entries per row of kept and weights_out that are written
 };
 
 // Weights as unsigned integers in the same order: NaN below everything, the two zeros equal.
@@ -41,129 +40,220 @@ __device__ __forceinline__ uint32_t weight_key(float f) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// Inclusive scan over the workgroup of a packed pair of counts (no carry between the halves: tiles hold 4096 tokens).
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *sm_wave, uint32_t &total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t up = __shfl_up(v, o, 64);
-        if (lane >= o) v += up;
-    }
-    if (lane == 63) sm_wave[wave] = v;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kSelectThreads / 64; ++w) {
-        const uint32_t c = sm_wave[w];
-        if (w < wave) before += c;
-        all += c;
-    }
-    total = all;
-    __syncthreads();  // sm_wave may be written again
-    return v + before;
+// Inclusive sum over the wavefront's lanes on the vector pipe (row shifts inside sixteen lanes, then the broadcasts of
+// lane 15 and of lane 31): six dependent additions instead of six trips through the LDS crossbar.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+#define HS_DPP_ADD(ctrl, rows) v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xf, false)
+    HS_DPP_ADD(0x111, 0xf);  // row_shr:1
+    HS_DPP_ADD(0x112, 0xf);  // row_shr:2
+    HS_DPP_ADD(0x114, 0xf);  // row_shr:4
+    HS_DPP_ADD(0x118, 0xf);  // row_shr:8
+    HS_DPP_ADD(0x142, 0xa);  // row_bcast:15 into rows 1 and 3
+    HS_DPP_ADD(0x143, 0xc);  // row_bcast:31 into rows 2 and 3
+#undef HS_DPP_ADD
+    return v;
 }
-
-__global__ __launch_bounds__(kSelectThreads) void evict_select_kernel(EvictArgs a) {
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+// One workgroup per row.  A thread owns four neighbouring weights of every 4 THREADS and keeps the keys of 4 NV of them in
+// registers, so a row of up to 4 NV THREADS tokens is read once, all loads in flight together, and the passes run on
+// registers; a longer row is read again for every pass, a tile of that length at a time.  Protected tokens take the
+// largest key, so every pass is one comparison per token.  What a row costs is the latency of its steps (three
+// histograms with a scan each, one scan for the list), so the scans run on the vector pipe and few waves take part in
+// a barrier: four for rows of up to 8192 tokens, sixteen beyond.
+constexpr int kSelectNV = 8;
+constexpr uint32_t kProtected = 0xffffffffu, kZeroKey = 0x80000000u;
+template <int THREADS>
+__global__ __launch_bounds__(THREADS, 4) void evict_select_kernel(EvictArgs a) {
+    constexpr int NV = kSelectNV, kWaves = THREADS / 64, kTile = NV * 4 * THREADS, BPT = 2048 / THREADS, kCounts = NV * kWaves;
+    static_assert(kCounts <= 128, "two counts per lane");
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t row = (int64_t)b * a.Hkv + h;
     const int L = min(max(a.seq_lens[b], 0), a.max_seq_len);
     const float *w = a.w ? a.w + row * a.w_stride : nullptr;
-    float *wo = a.wo ? a.wo + row * a.wo_stride : nullptr;
-    int32_t *list = a.list + row * a.budget, *kept = a.kept ? a.kept + row * a.budget : nullptr;
-    __shared__ uint32_t sm_hist[2048], sm_wave[kSelectThreads / 64], sm_pick[3];
+    int32_t *list = a.list + row * a.budget;
+    __shared__ __attribute__((aligned(16))) uint32_t sm_hist[3][2048];
+    __shared__ uint32_t sm_wave[kWaves], sm_pick[3][2], sm_cnt[kCounts];
+    __shared__ int sm_first;
     const int n = min(L, a.budget);
-    int first_moved = n;
     if (L <= a.budget || w == nullptr) {
         // nothing to choose: everything, or the sinks and the newest
         const int s = L <= a.budget ? n : a.sinks;
-        for (int i = tid; i < a.budget; i += kSelectThreads) {
-            const int t = i < s ? i : L - n + i;
-            if (i < n) list[i] = t;
-            if (kept) kept[i] = i < n ? t : -1;
-            if (wo && i < n && !(w == wo)) wo[i] = w ? w[t] : 0.0f;
-        }
-        first_moved = L <= a.budget ? n : a.sinks;
+        for (int i = tid; i < n; i += THREADS) list[i] = i < s ? i : L - n + i;
+        if (tid == 0) sm_first = s;
     } else {
         const int lo = a.sinks, hi = L - a.recent, K = a.budget - a.sinks - a.recent;
+        const int tiles = (L + kTile - 1) / kTile;
+        float4v x[NV];
+        uint32_t key[NV][4];  // tokens behind the row take key 0: the lowest one, and last among its equals
+        auto load = [&](int tile) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int t0 = tile * kTile + 4 * (i * THREADS + tid);
+                x[i] = t0 < L ? *(const float4v *)(w + t0) : (float4v){0.f, 0.f, 0.f, 0.f};  // rows are a multiple of four long
+            }
+        };
+        auto make_keys = [&](int tile) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int t0 = tile * kTile + 4 * (i * THREADS + tid);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int t = t0 + e;
+                    key[i][e] = t >= L ? 0u : t < lo || t >= hi ? kProtected : weight_key(x[i][e]);
+                }
+            }
+        };
+        // groups of four tokens per thread that lie in the row (uniform over the workgroup)
+        auto groups = [&](int tile) { return min(NV, (L - tile * kTile + 4 * THREADS - 1) / (4 * THREADS)); };
+        load(0);
+        for (int i = tid; i < 3 * 2048 / 4; i += THREADS) ((u32x4 *)&sm_hist[0][0])[i] = (u32x4){0u, 0u, 0u, 0u};
+        if (tid == 0) sm_first = n;
+        __syncthreads();
+        make_keys(0);
         // ---- key of the K-th heaviest token of [lo, hi), three digits of 11, 11 and 10 bits; `need` of those that share
         //      it stay, the lowest positions first
-        uint32_t prefix = 0, need = (uint32_t)K;
+        uint32_t prefix = kProtected - 1, need = 0;
         if (K > 0) {
-            const int shift[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
+            constexpr int shift[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
+            constexpr uint32_t mask[3] = {2047u, 2047u, 1023u};
+            prefix = 0;
+            need = (uint32_t)K;
 #pragma unroll
             for (int p = 0; p < 3; ++p) {
-                for (int i = tid; i < 2048; i += kSelectThreads) sm_hist[i] = 0;
-                __syncthreads();
-                const uint32_t mask = (1u << bits[p]) - 1;
-                for (int t = lo + tid; t < hi; t += kSelectThreads) {
-                    const uint32_t k = weight_key(w[t]);
-                    if (p == 0 || (k >> (shift[p] + bits[p])) == (prefix >> (shift[p] + bits[p]))) atomicAdd(&sm_hist[(k >> shift[p]) & mask], 1u);
+                uint32_t zeros = 0;  // tokens without any weight are many and would queue at one counter
+                for (int tile = 0; tile < tiles; ++tile) {
+                    if (tiles > 1) {
+                        load(tile);
+                        make_keys(tile);
+                    }
+                    const int ng = groups(tile);
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) {
+                        if (i >= ng) break;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t k = key[i][e];
+                            if (p == 0 && k == kZeroKey) ++zeros;
+                            else if (k != kProtected && (p == 0 || ((k ^ prefix) >> (shift[p] + bits[p])) == 0u))
+                                atomicAdd(&sm_hist[p][(k >> shift[p]) & mask[p]], 1u);
+                        }
+                    }
+                }
+                if (p == 0) {
+                    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(zeros), 63);
+                    if (lane == 0 && all != 0) atomicAdd(&sm_hist[0][kZeroKey >> 21], all);
                 }
                 __syncthreads();
-                // the digit at which the count from the top reaches `need`: thread i owns the two bins below 2048 - 2 i
-                const int top = 2047 - 2 * tid;
-                const uint32_t c1 = sm_hist[top], c0 = sm_hist[top - 1];
-                uint32_t all;
-                const uint32_t incl = block_scan(c1 + c0, sm_wave, all), excl = incl - c1 - c0;
+                // the digit at which the count from the top reaches `need`: thread i owns the BPT bins below 2048 - BPT i
+                uint32_t bin[BPT], sum = 0;
+#pragma unroll
+                for (int e = 0; e < BPT; ++e) bin[e] = sm_hist[p][2048 - BPT * (tid + 1) + e];
+#pragma unroll
+                for (int e = 0; e < BPT; ++e) sum += bin[e];
+                uint32_t incl = wave_scan(sum);
+                if (lane == 63) sm_wave[wave] = incl;
+                __syncthreads();
+                const uint32_t totals = wave_scan(lane < kWaves ? sm_wave[lane] : 0u);
+                if (wave > 0) incl += (uint32_t)__builtin_amdgcn_readlane((int)totals, wave - 1);
+                uint32_t excl = incl - sum;
                 if (excl < need && need <= incl) {
-                    const bool upper = excl + c1 >= need;
-                    sm_pick[0] = upper ? top : top - 1;
-                    sm_pick[1] = need - excl - (upper ? 0u : c1);
+#pragma unroll
+                    for (int e = BPT - 1; e >= 0; --e) {
+                        if (excl < need && need <= excl + bin[e]) {
+                            sm_pick[p][0] = (uint32_t)(2048 - BPT * (tid + 1) + e);
+                            sm_pick[p][1] = need - excl;
+                        }
+                        excl += bin[e];
+                    }
                 }
                 __syncthreads();
-                prefix |= sm_pick[0] << shift[p];
-                need = sm_pick[1];
-                __syncthreads();
+                prefix |= sm_pick[p][0] << shift[p];
+                need = sm_pick[p][1];
             }
         }
-        // ---- list, in order.  A token stays if it is protected, heavier than the key, or one of the first `need` at it.
+        // ---- list, in order.  A token stays if its key is larger, or one of the first `need` equal ones.
+        //      Counts travel in pairs: larger ones in the low half, ties in the high one (a tile holds at most 32768).
+        float *wo = a.w == a.wo ? a.wo + row * a.wo_stride : nullptr;  // in place; otherwise they move with their tokens
         uint32_t sure = 0, ties = 0;  // of the tiles before this one
-        const int tiles = (L + 4 * kSelectThreads - 1) / (4 * kSelectThreads);
         for (int tile = 0; tile < tiles; ++tile) {
-            const int t0 = tile * 4 * kSelectThreads + 4 * tid;
-            float4v x = {0.f, 0.f, 0.f, 0.f};
-            if (t0 < L) x = *(const float4v *)(w + t0);  // rows are a multiple of four long
-            uint32_t own[4], cnt = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int t = t0 + e;
-                const uint32_t k = weight_key(x[e]);
-                const bool prot = t < L && (t < lo || t >= hi);
-                const bool mid = K > 0 && t >= lo && t < hi;
-                own[e] = prot || (mid && k > prefix) ? 1u : (mid && k == prefix ? 0x10000u : 0u);
-                cnt += own[e];
+            if (tiles > 1) {
+                load(tile);
+                make_keys(tile);
             }
-            uint32_t all;
-            uint32_t at = block_scan(cnt, sm_wave, all) - cnt;
-            uint32_t s = sure + (at & 0xffffu), q = ties + (at >> 16);
+            const int ng = groups(tile);
+            uint32_t below[NV];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const bool stays = own[e] == 1u || (own[e] == 0x10000u && q < need);
-                if (stays) {
-                    const int r = (int)(s + min(q, need));
-                    list[r] = t0 + e;
-                    if (kept) kept[r] = t0 + e;
-                    if (wo) wo[r] = x[e];  // in place: r <= t0 + e, and this tile has been read
-                    if (r != t0 + e) first_moved = min(first_moved, r);
+            for (int i = 0; i < NV; ++i) {
+                uint32_t cnt = 0;
+                if (i < ng) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) cnt += key[i][e] > prefix ? 1u : key[i][e] == prefix ? 0x10000u : 0u;
                 }
-                s += own[e] & 1u;
-                q += own[e] >> 16;
+                const uint32_t incl = wave_scan(cnt);
+                if (lane == 63) sm_cnt[i * kWaves + wave] = incl;
+                below[i] = incl - cnt;
             }
+            __syncthreads();
+            // counts in the order of the tokens: entry i * kWaves + wave.  Every wavefront sums them up for itself.
+            uint32_t c0 = 0, c1 = 0;
+            if (2 * lane < kCounts) {
+                c0 = sm_cnt[2 * lane];
+                c1 = sm_cnt[2 * lane + 1];
+            }
+            const uint32_t pair = wave_scan(c0 + c1);
+            __syncthreads();  // sm_cnt may be written again; with weights in place: this tile has been read everywhere
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if (i >= ng) break;
+                const int at = i * kWaves + wave;
+                uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)pair, at >> 1) - (uint32_t)__builtin_amdgcn_readlane((int)c1, at >> 1);
+                if (!(at & 1)) before -= (uint32_t)__builtin_amdgcn_readlane((int)c0, at >> 1);
+                before += below[i];
+                uint32_t s = sure + (before & 0xffffu), q = ties + (before >> 16);
+                const int t0 = tile * kTile + 4 * (i * THREADS + tid);
+                bool gap = false;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool is_sure = key[i][e] > prefix, is_tie = key[i][e] == prefix;
+                    if (is_sure || (is_tie && q < need)) {
+                        const int r = (int)(s + min(q, need));
+                        list[r] = t0 + e;
+                        if (wo) wo[r] = x[i][e];  // r <= t, and this tile has been read
+                    } else {
+                        gap = true;
+                    }
+                    s += is_sure ? 1u : 0u;
+                    q += is_tie ? 1u : 0u;
+                }
+                // the first list entry that moves is the first token that leaves; a lower bound at four tokens' grain
+                const uint64_t gaps = __builtin_amdgcn_ballot_w64(gap);
+                if (gaps != 0 && lane == 0) atomicMin(&sm_first, tile * kTile + 4 * (i * THREADS + 64 * wave + __builtin_ctzll(gaps)));
+            }
+            const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)pair, 63);
             sure += all & 0xffffu;
             ties += all >> 16;
         }
     }
-    // ---- the tail of the weights and of the list, the row's counts
+    // ---- weights in place: the tail; the row's counts
     __syncthreads();
-    if (wo)
-        for (int64_t i = n + tid; i < min(a.wo_stride, (int64_t)a.max_seq_len); i += kSelectThreads) wo[i] = 0.0f;
-    if (tid == 0) sm_pick[2] = (uint32_t)n;
-    __syncthreads();
-    atomicMin(&sm_pick[2], (uint32_t)first_moved);
-    __syncthreads();
+    if (a.w && a.w == a.wo)
+        for (int64_t i = n + tid; i < min(a.wo_stride, (int64_t)a.max_seq_len); i += THREADS) a.wo[row * a.wo_stride + i] = 0.0f;
     if (tid == 0) {
         a.info[2 * row] = n;
-        a.info[2 * row + 1] = (int)sm_pick[2];
+        a.info[2 * row + 1] = min(sm_first, n);
+    }
+}
+
+// What goes with the codes of list entries [i0, i1): the caller's list, the weights and the zeros behind them (weights in
+// place have been moved by the selection).  `threads` threads take part.
+__device__ __forceinline__ void finish_rows(const EvictArgs &a, int64_t row, int n, int i0, int i1, int tid, int threads) {
+    const int32_t *list = a.list + row * a.budget;
+    const bool move_weights = a.wo != nullptr && a.w != a.wo;
+    if (!move_weights && a.kept == nullptr) return;
+    const int64_t w_end = min(a.wo_stride, (int64_t)a.max_seq_len);
+    for (int i = i0 + tid; i < i1; i += threads) {
+        const int t = i < n ? list[i] : -1;
+        if (a.kept && i < a.budget) a.kept[row * a.budget + i] = t;
+        if (move_weights && i < w_end) a.wo[row * a.wo_stride + i] = t >= 0 && a.w ? a.w[row * a.w_stride + t] : 0.0f;
     }
 }
 
@@ -178,6 +268,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
     if (blockIdx.x == 0 && h == 0 && tid == 0) a.seq_lens_out[b] = n;
     if (blockIdx.x == 0 && a.fp8 && tid < 2) (tid ? a.vso : a.kso)[row] = (tid ? a.vs : a.ks)[row];
     const int i0 = blockIdx.x * kMoveTokens;
+    finish_rows(a, row, n, i0, i0 + kMoveTokens, tid, 256);
     if (i0 >= n) return;
     const int32_t *list = a.list + row * a.budget;
     const int sub = tid % LPR, r = tid / LPR;
@@ -228,6 +319,7 @@ __global__ __launch_bounds__(1024) void evict_inplace_kernel(EvictArgs a) {
     const int64_t row = (int64_t)b * a.Hkv + h;
     const int n = a.info[2 * row], first = a.info[2 * row + 1];
     if (which == 0 && h == 0 && tid == 0) a.seq_lens_out[b] = n;
+    if (which == 0) finish_rows(a, row, n, 0, a.finish, tid, 1024);
     const int32_t *list = a.list + row * a.budget;
     const KvAddr &ad = which ? a.va : a.ka;
     uint8_t *codes = which ? a.vco : a.kco;
@@ -356,8 +448,11 @@ int hs_kv_evict(int fmt_fp8, const void *k_codes, const void *v_codes, const flo
     a.info = a.list + (size_t)B * Hkv * budget;
     a.budget = budget; a.sinks = sinks; a.recent = recent;
     a.Hkv = Hkv; a.D = D; a.max_seq_len = max_seq_len; a.fp8 = fp8 ? 1 : 0;
+    a.finish = std::max(std::min(budget, max_seq_len), kept ? budget : 0);
+    if (weights_out) a.finish = std::max<int64_t>(a.finish, std::min<int64_t>(weights_out_stride, max_seq_len));
     hipStream_t st = (hipStream_t)stream;
-    evict_select_kernel<<<dim3(Hkv, B), kSelectThreads, 0, st>>>(a);
+    if (max_seq_len <= 4 * kSelectNV * 256) evict_select_kernel<256><<<dim3(Hkv, B), 256, 0, st>>>(a);
+    else evict_select_kernel<1024><<<dim3(Hkv, B), 1024, 0, st>>>(a);
     if (int rc = check_launch("kv_evict (selection)")) return rc;
     if (in_place) {
         const dim3 grid(2, Hkv, B);
@@ -365,7 +460,7 @@ int hs_kv_evict(int fmt_fp8, const void *k_codes, const void *v_codes, const flo
         else if (D == 128) evict_inplace_kernel<128><<<grid, 1024, 0, st>>>(a);
         else evict_inplace_kernel<256><<<grid, 1024, 0, st>>>(a);
     } else {
-        const dim3 grid((std::min(budget, max_seq_len) + kMoveTokens - 1) / kMoveTokens, Hkv, B);
+        const dim3 grid((a.finish + kMoveTokens - 1) / kMoveTokens, Hkv, B);
         if (D == 64) evict_move_kernel<64><<<grid, 256, 0, st>>>(a);
         else if (D == 128) evict_move_kernel<128><<<grid, 256, 0, st>>>(a);
         else evict_move_kernel<256><<<grid, 256, 0, st>>>(a);
