@@ -14,14 +14,21 @@
 // The keys sit on the M axis, so a lane's four score registers are four keys of one column: row statistics stay in the
 // lane until the end of the walk, and so do the column sums.
 #include <algorithm>
+#include <climits>
+#include <type_traits>
 
 #include "mfma_common.hpp"
 
 namespace hs {
 
 constexpr float kWLog2e = 1.4426950408889634f;
-constexpr int kWStep = 64;       // keys of a step (first kernel), columns of a step (second)
-constexpr int kWSegment = 2048;  // columns of a workgroup of the second kernel, at most
+constexpr int kWStep = 64;       // keys of a step of the first kernel
+#ifndef CHN
+#define CHN 1024
+#define CHM 512
+#endif
+constexpr int kCStepMax = 128;   // columns of a step of the second (64 at head_dim 256)
+constexpr int kWThreads = 256;   // both kernels
 
 struct WeightsArgs {
     const uint16_t *q;   // [B, S, Hq, D] bf16
@@ -33,11 +40,11 @@ struct WeightsArgs {
     float *out;
     int64_t stride;
     float *part_ml;      // [B, Hkv, key chunks, columns, 2]
-    float *lse;          // [B, Hkv, columns], log2 units; +inf = the column sees nothing
+    float *lse;          // [B, Hkv, lse_stride], log2 units; +inf = the column sees nothing, or there is none
     float *part_w;       // [segments, B, Hkv, part_stride] when the columns of a key block are split
     int64_t part_stride;
     int32_t start_pos, B, S, Hq, Hkv, G, cols, max_seq_len, window, sinks;
-    int32_t key_chunks, chunk_tokens, segments;
+    int32_t key_chunks, chunk_tokens, segments, lse_stride;
     float scale_log2e;
 };
 
@@ -49,47 +56,98 @@ __device__ __forceinline__ int first_pos(const WeightsArgs &a, int b) {
 __device__ __forceinline__ int key_count(const WeightsArgs &a, int pos0) {
     return (int)min((int64_t)a.max_seq_len, max((int64_t)0, (int64_t)pos0 + a.S));
 }
-__device__ __forceinline__ bool sees(const WeightsArgs &a, int p, int t) {  // p already inside [0, max_seq_len)
-    return t <= p && (a.window == 0 || t > p - a.window || t < a.sinks);
+// Does a query at p (inside [0, max_seq_len), or negative: no query) see token t?  lo: below which tokens are out of the
+// window (INT_MIN without one).  No branches: this runs for every score of a step that is cut by a bound.
+__device__ __forceinline__ bool sees(int p, int lo, int sinks, int t) {
+    return (t <= p) & ((t > lo) | (t < sinks));
+}
+__device__ __forceinline__ int window_lo(const WeightsArgs &a, int p) { return a.window == 0 ? INT_MIN : p - a.window; }
+
+// Memory straight to LDS, 16 or 4 bytes a lane: lane i's go to dst + 16 i (4 i), dst uniform over the wavefront.
+typedef __attribute__((address_space(3))) void *lds_ptr;
+__device__ __forceinline__ void copy16_to_lds(const void *src, void *dst) { __builtin_amdgcn_global_load_lds(src, (lds_ptr)dst, 16, 0, 0); }
+__device__ __forceinline__ void copy4_to_lds(const void *src, void *dst) { __builtin_amdgcn_global_load_lds(src, (lds_ptr)dst, 4, 0, 0); }
+
+// Sum over the sixteen lanes of a row, in every one of them (rotations inside the row).
+__device__ __forceinline__ float row_sum(float x) {
+#define HS_ROR_ADD(n) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + n, 0xf, 0xf, false))
+    HS_ROR_ADD(8);
+    HS_ROR_ADD(4);
+    HS_ROR_ADD(2);
+    HS_ROR_ADD(1);
+#undef HS_ROR_ADD
+    return x;
 }
 
-// e4m3fn code -> bf16 bits (exact)
-__device__ __forceinline__ uint32_t e4m3_to_bf16(uint32_t c) {
-    const half2v h = __builtin_bit_cast(half2v, e4m3_high_bytes_to_f16(c << 8));  // value / 256 in the low half
-    return __float_as_uint((float)h[0] * 256.0f) >> 16;
-}
-__device__ __forceinline__ uint32_t code_to_bf16(uint32_t c, bool fp8) {
-    return fp8 ? e4m3_to_bf16(c) : __float_as_uint((float)(int8_t)c) >> 16;
+// Eight codes (two dwords) -> eight bf16, exactly.
+template <bool FP8>
+__device__ __forceinline__ bf16x8 codes_to_bf16(uint32_t w0, uint32_t w1) {
+    uint32_t o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = i < 2 ? w0 : w1;
+        float lo, hi;
+        if constexpr (FP8) {
+            const auto f = (i & 1) ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+            lo = f[0];
+            hi = f[1];
+        } else {
+            lo = (float)(int8_t)(w >> (16 * (i & 1)));
+            hi = (float)(int8_t)(w >> (16 * (i & 1) + 8));
+        }
+        o[i] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);  // the upper halves
+    }
+    return pack_bf16x8(o[0], o[1], o[2], o[3]);
 }
 
-template <int D, bool FP8>
-__global__ __launch_bounds__(256, 2) void weights_stats_kernel(WeightsArgs a) {
-    constexpr int KG = D / 32, TPR = D / 32, RPP = 256 / TPR;  // threads per key row (32 codes each), rows per pass
-    constexpr int PASSES = RPP >= kWStep ? 1 : kWStep / RPP;
-    constexpr int NB = D == 256 ? 2 : 4;                       // 16-column blocks of a wavefront
+// Address of token t's codes and scale (uniform over the wavefront; `span` tokens from there lie in one block).
+struct KeyBase {
+    const uint8_t *codes;
+    const float *scales;
+};
+__device__ __forceinline__ KeyBase key_base(const WeightsArgs &a, int b, int h, int t, int D, bool fp8) {
+    int64_t u;
+    int slot;
+    resolve(a.ka, b, t, u, slot);
+    KeyBase k;
+    k.codes = a.kc + u * a.ka.code_stride_seq + (int64_t)h * a.ka.code_stride_head + (int64_t)slot * D;
+    k.scales = fp8 ? nullptr : a.ks + u * a.ka.scale_stride_seq + (int64_t)h * a.ka.scale_stride_head + slot;
+    return k;
+}
+
+// NB: 16-column blocks of a wavefront (its columns stay in registers as B operands).  Per 16 keys a wavefront reads the
+// K operands once from LDS and multiplies all its columns with them; a lane keeps a running (m, l) of its own keys of
+// each column, m a bound that overshoots (as in the prefill kernel) so that most steps only check it.
+template <int D, bool FP8, int NB>
+__global__ __launch_bounds__(kWThreads, 2) void weights_stats_kernel(WeightsArgs a) {
+    constexpr int KG = D / 32, TPR = D / 16, RPP = kWThreads / TPR;  // threads per key row (16 codes each), rows per pass
+    constexpr int PASSES = RPP >= kWStep ? 1 : kWStep / RPP, WGC = kWThreads / 4 * NB;  // columns of the workgroup
+    constexpr float kOver = 8.0f;  // log2 units by which the bound overshoots a new maximum
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lq = lane >> 4;
     const int units = a.B * a.Hkv;
     // units are the fastest index: the workgroups that stream one unit's keys share an XCD and its L2
     const int unit = blockIdx.x % units, chunk = (blockIdx.x / units) % a.key_chunks;
-    const int blk = (int)((a.cols + 64 * NB - 1) / (64 * NB)) - 1 - (int)(blockIdx.x / units / a.key_chunks);  // late columns first: they see most
+    const int blk = (int)((a.cols + WGC - 1) / WGC) - 1 - (int)(blockIdx.x / units / a.key_chunks);  // late columns first: they see most
     const int b = unit / a.Hkv, h = unit % a.Hkv;
     const int pos0 = first_pos(a, b);
-    const int wg_c0 = blk * 64 * NB, wg_c1 = min(a.cols, wg_c0 + 64 * NB) - 1;
+    const int wg_c0 = blk * WGC, wg_c1 = min(a.cols, wg_c0 + WGC) - 1, wv_c0 = wg_c0 + 16 * NB * wave;
     const int T = key_count(a, pos0);
-    __shared__ __attribute__((aligned(16))) uint8_t sm_k[2][4 * KG][1024];  // block KG u + j: keys 16u .., d 32j ..; operand order
+    // block KG u + j: the operand of keys 16u .. and d 32j ..; its 16-byte piece of lane (li, lq) sits at piece
+    // 16 lq + (li ^ (2j + lq / 2)), which spreads the eight pieces a key row writes at once over the banks
+    __shared__ __attribute__((aligned(16))) uint8_t sm_k[2][4 * KG][1024];
+    const int piece = 16 * lq + (li ^ (lq >> 1));
     __shared__ __attribute__((aligned(16))) float sm_s[2][kWStep];
 
-    // ---- columns: lane (li, lq) holds column li of each block, d = 32j + 8 lq + e
+    // ---- columns: lane (li, lq) holds column li of each block, d = 32j + 8 lq + e, as fp16 times a power of two.  One
+    //      power for the blocks of a lane (it then goes into the keys' scales) while their magnitudes are within 2^4 of
+    //      each other, else (`own`) one per column.
     half8 qop[NB][KG];
     float cq[NB], m[NB], l[NB];
-    int pos[NB];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-        const int c = wg_c0 + 16 * NB * wave + 16 * nb + li, cc = min(c, a.cols - 1);
-        const int s = cc / a.G, g = cc % a.G;
+    int pos[NB], ex[NB], ex_hi = -1000, ex_lo = 1000;
+    auto load_q = [&](int nb, float (&qf)[8 * KG]) {
+        const int c = min(wv_c0 + 16 * nb + li, a.cols - 1), s = c / a.G, g = c % a.G;
         const uint16_t *qp = a.q + (((int64_t)b * a.S + s) * a.Hq + h * a.G + g) * D + 8 * lq;
-        float qf[8 * KG], amax = 0.0f;
 #pragma unroll
         for (int j = 0; j < KG; ++j) {
             const u32x4 w = *(const u32x4 *)(qp + 32 * j);
@@ -99,22 +157,36 @@ __global__ __launch_bounds__(256, 2) void weights_stats_kernel(WeightsArgs a) {
                 qf[8 * j + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
             }
         }
+        return pos0 + s;
+    };
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        float qf[8 * KG], amax = 0.0f;
+        const int p = load_q(nb, qf);
 #pragma unroll
         for (int i = 0; i < 8 * KG; ++i) amax = fmaxf(amax, fabsf(qf[i]));
         amax = quad_max(amax);
-        // amax = f 2^ex with f in [0.5, 1): the power of two comes off the operands and goes back into the scale, exactly
-        int ex = 0;
-        if (amax > 0.0f && amax < 3.0e38f) ex = min(126, max(-125, (int)((__float_as_uint(amax) >> 23) & 0xff) - 126));
-        const float down = __uint_as_float((uint32_t)(127 - ex) << 23), up = __uint_as_float((uint32_t)(127 + ex) << 23);
+        // amax = f 2^ex with f in [0.5, 1)
+        ex[nb] = 0;
+        if (amax > 0.0f && amax < 3.0e38f) ex[nb] = min(126, max(-125, (int)((__float_as_uint(amax) >> 23) & 0xff) - 126));
+        ex_hi = max(ex_hi, ex[nb]);
+        ex_lo = min(ex_lo, ex[nb]);
+        pos[nb] = wv_c0 + 16 * nb + li < a.cols && p < a.max_seq_len ? p : -1;  // a column that sees nothing (p < 0 included)
+        m[nb] = 0.0f;
+        l[nb] = 0.0f;
+    }
+    const bool own = NB > 1 && __builtin_amdgcn_ballot_w64(ex_hi - ex_lo > 4) != 0;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        if (!own) ex[nb] = ex_hi;
+        const float down = __uint_as_float((uint32_t)(127 - ex[nb]) << 23), up = __uint_as_float((uint32_t)(127 + ex[nb]) << 23);
+        float qf[8 * KG];
+        load_q(nb, qf);
 #pragma unroll
         for (int j = 0; j < KG; ++j)
 #pragma unroll
             for (int e = 0; e < 8; ++e) qop[nb][j][e] = (_Float16)(qf[8 * j + e] * down);
         cq[nb] = a.scale_log2e * up * (FP8 ? 256.0f : 1.0f);  // e4m3fn operands are value / 256
-        const int p = pos0 + s;
-        pos[nb] = c < a.cols && p < a.max_seq_len ? p : -1;   // a column that sees nothing (p < 0 included)
-        m[nb] = -INFINITY;
-        l[nb] = 0.0f;
     }
     const float head_scale = FP8 ? a.ks[(int64_t)b * a.Hkv + h] : 0.0f;
 
@@ -127,31 +199,19 @@ __global__ __launch_bounds__(256, 2) void weights_stats_kernel(WeightsArgs a) {
     const int s_hi = c_hi > c_lo ? (c_hi + kWStep - 1) / kWStep : 0;
     int st = next_step(c_lo / kWStep);
 
-    u32x4 raw[PASSES][2];
-    float rawsc = 0.0f;
+    u32x4 raw[PASSES];
+    float rawsc = head_scale;
     const int krow = tid / TPR, kq = tid % TPR;
     auto load = [&](int step) {
-        const int t0 = step * kWStep;
+        const int t0 = step * kWStep, last = T - 1 - t0;
+        const KeyBase k = key_base(a, b, h, t0, D, FP8);
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
-            int64_t ku;
-            int slot;
             const int row = krow + p * RPP;
             if (RPP > kWStep && row >= kWStep) continue;
-            resolve(a.ka, b, min(t0 + row, T - 1), ku, slot);
-            const u32x4 *src = (const u32x4 *)(a.kc + ku * a.ka.code_stride_seq + (int64_t)h * a.ka.code_stride_head + (int64_t)slot * D + 32 * kq);
-            raw[p][0] = src[0];
-            raw[p][1] = src[1];
+            raw[p] = *(const u32x4 *)(k.codes + (uint32_t)(min(row, last) * D + 16 * kq));
         }
-        if (tid < kWStep) {
-            if (FP8) rawsc = head_scale;
-            else {
-                int64_t ku;
-                int slot;
-                resolve(a.ka, b, min(t0 + tid, T - 1), ku, slot);
-                rawsc = a.ks[ku * a.ka.scale_stride_seq + (int64_t)h * a.ka.scale_stride_head + slot];
-            }
-        }
+        if (!FP8 && tid < kWStep) rawsc = k.scales[min(tid, last)];
     };
     auto commit = [&](int buf) {
         const _Float16 bias = (_Float16)1152.0f;
@@ -159,75 +219,153 @@ __global__ __launch_bounds__(256, 2) void weights_stats_kernel(WeightsArgs a) {
         for (int p = 0; p < PASSES; ++p) {
             const int row = krow + p * RPP;
             if (RPP > kWStep && row >= kWStep) continue;
-            uint8_t *dst = sm_k[buf][KG * (row >> 4) + kq] + (row & 15) * 16;
+            // codes 16 kq ..: d-group j = kq / 2, lane groups lq = 2 (kq % 2) and the next
+            uint8_t *dst = sm_k[buf][KG * (row >> 4) + (kq >> 1)] + (32 * (kq & 1) + ((row & 15) ^ (2 * (kq >> 1) + (kq & 1)))) * 16;
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-                const uint32_t w0 = raw[p][q4 >> 1][2 * (q4 & 1)], w1 = raw[p][q4 >> 1][2 * (q4 & 1) + 1];
-                *(half8 *)(dst + 256 * q4) = FP8 ? e4m3x8_to_f16_div256(w0, w1) : int8x8_to_f16_biased(w0, w1) - bias;
+            for (int q2 = 0; q2 < 2; ++q2) {
+                const uint32_t w0 = raw[p][2 * q2], w1 = raw[p][2 * q2 + 1];
+                *(half8 *)(dst + 256 * q2) = FP8 ? e4m3x8_to_f16_div256(w0, w1) : int8x8_to_f16_biased(w0, w1) - bias;
             }
         }
         if (tid < kWStep) sm_s[buf][tid] = rawsc;
     };
-    const int wave_first = pos0 + (wg_c0 + 16 * NB * wave) / a.G, wave_last = pos0 + min(a.cols - 1, wg_c0 + 16 * NB * wave + 16 * NB - 1) / a.G;
-    const bool active = wg_c0 + 16 * NB * wave < a.cols;
+    const int wave_first = pos0 + wv_c0 / a.G, wave_last = pos0 + min(a.cols - 1, wv_c0 + 16 * NB - 1) / a.G;
+    const bool active = wv_c0 < a.cols, ragged = wave_last >= a.max_seq_len || wave_first < 0 || wv_c0 + 16 * NB > a.cols;
+    bool force = true;  // some column has no bound yet
     if (st < s_hi) {
         load(st);
         commit(0);
     }
     __syncthreads();
-    for (int buf = 0; st < s_hi; buf ^= 1) {
-        const int nst = next_step(st + 1);
-        if (nst < s_hi) load(nst);
-        const int t0 = st * kWStep;
-        if (active && t0 <= wave_last) {
-            // some (key, column) pair of the step may be hidden: in the future, out of the window, past the chunk or in no sequence
-            const bool edge = t0 + kWStep - 1 > wave_first || wave_last >= a.max_seq_len || wave_first < 0 || (a.window && t0 <= wave_last - a.window) ||
-                              (wg_c1 + 1 == a.cols && wg_c0 + 16 * NB * (wave + 1) > a.cols);
+    auto walk = [&](auto own_tag) {
+        constexpr bool kOwn = decltype(own_tag)::value;
+        for (int buf = 0; st < s_hi; buf ^= 1) {
+            const int nst = next_step(st + 1);
+            if (nst < s_hi) load(nst);
+            const int t0 = st * kWStep;
+            if (active && t0 <= wave_last) {
+                // some (key, column) pair of the step may be hidden: in the future, out of the window or in no sequence
+                const bool edge = t0 + kWStep - 1 > wave_first || ragged || (a.window && t0 <= wave_last - a.window);
+                // A step without hidden pairs, once every column has a bound: no score is compared with it.  The bound only
+                // keeps the exponentials in range; a score that passes it by less than kFar is as good as any, and a step
+                // with one beyond is done again with the comparing form.  Operands are read kAhead blocks ahead through a
+                // ring, the exponentials of sixteen keys are made among the products of the next, in a pinned order.
+                auto consume_fast = [&]() {
+                    constexpr int kAhead = 4, kRing = 8, kBlocks = 4 * KG;
+                    constexpr float kFar = 64.0f;
+                    float4v acc[2][NB], sk[2];
+                    half8 ring[kRing];
+                    float l_old[NB], pend = 0.0f;
+                    int over = INT_MIN, last_x = INT_MIN;
+                    auto read = [&](int k) { return *(const half8 *)(sm_k[buf][k] + (piece ^ (2 * (k % KG))) * 16); };
+                    auto weight = [&](int u, int e) {  // e = 4 nb + r
+                        if (e > 0) l[(e - 1) >> 2] += pend;
+                        const float x = acc[u & 1][e >> 2][e & 3] * sk[u & 1][e & 3] - m[e >> 2];
+                        if (e & 1) over = max(over, max(last_x, __float_as_int(x)));  // positive floats order like their bits
+                        last_x = __float_as_int(x);
+                        pend = __builtin_amdgcn_exp2f(x);
+                    };
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                float sc[16];
+                    for (int nb = 0; nb < NB; ++nb) l_old[nb] = l[nb];
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    float4v acc = {0.f, 0.f, 0.f, 0.f};
+                    for (int k = 0; k < kAhead; ++k) ring[k] = read(k);
 #pragma unroll
-                    for (int j = 0; j < KG; ++j)
-                        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(*(const half8 *)(sm_k[buf][KG * u + j] + lane * 16), qop[nb][j], acc, 0, 0, 0);
-                    const float4v sk = *(const float4v *)&sm_s[buf][16 * u + 4 * lq];
+                    for (int k = 0; k < kBlocks; ++k) {
+                        const int u = k / KG, j = k % KG;
+                        if (k + kAhead < kBlocks) ring[(k + kAhead) % kRing] = read(k + kAhead);
+                        if (j == 0) sk[u & 1] = *(const float4v *)&sm_s[buf][16 * u + 4 * lq] * cq[0];
+                        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) sc[4 * u + r] = acc[r] * sk[r] * cq[nb];
-                }
-                if (edge) {
+                        for (int nb = 0; nb < NB; ++nb) {
+                            acc[u & 1][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ring[k % kRing], qop[nb][j], j == 0 ? (float4v){0.f, 0.f, 0.f, 0.f} : acc[u & 1][nb], 0, 0, 0);
+                            if (u > 0) {
+                                const int i = j * NB + nb;  // product i of KG NB
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (!sees(a, pos[nb], t0 + 16 * (i >> 2) + 4 * lq + (i & 3))) sc[i] = -INFINITY;
-                }
-                float mx = sc[0];
+                                for (int e = i * 4 / KG; e < (i + 1) * 4 / KG; ++e) weight(u - 1, e);
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                        if (u > 0 && j == KG - 1) l[NB - 1] += pend;
+                    }
 #pragma unroll
-                for (int i = 1; i < 16; ++i) mx = fmaxf(mx, sc[i]);
-                if (__builtin_amdgcn_ballot_w64(mx > m[nb]) != 0) {
-                    const float m_new = fmaxf(m[nb], mx);
-                    if (m_new != -INFINITY) l[nb] *= __builtin_amdgcn_exp2f(m[nb] - m_new);
-                    m[nb] = m_new;
-                }
-                const float ref = m[nb] == -INFINITY ? 0.0f : m[nb];
+                    for (int e = 0; e < 4 * NB; ++e) weight(3, e);
+                    l[NB - 1] += pend;
+                    if (__builtin_amdgcn_ballot_w64(over > __float_as_int(kFar)) == 0) return true;
 #pragma unroll
-                for (int i = 0; i < 16; ++i) l[nb] += __builtin_amdgcn_exp2f(sc[i] - ref);
+                    for (int nb = 0; nb < NB; ++nb) l[nb] = l_old[nb];
+                    return false;
+                };
+                auto consume = [&](auto edge_tag) {
+                    constexpr bool kEdge = decltype(edge_tag)::value;
+                    float4v acc[NB];
+                    auto product = [&](int u) {
+#pragma unroll
+                        for (int j = 0; j < KG; ++j) {
+                            const half8 kop = *(const half8 *)(sm_k[buf][KG * u + j] + (piece ^ (2 * j)) * 16);
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb)
+                                acc[nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kop, qop[nb][j], j == 0 ? (float4v){0.f, 0.f, 0.f, 0.f} : acc[nb], 0, 0, 0);
+                        }
+                    };
+                    product(0);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        float4v sk = *(const float4v *)&sm_s[buf][16 * u + 4 * lq];
+                        if (!kOwn) sk *= cq[0];
+                        float e[NB][4];
+                        int over = force ? INT_MAX : INT_MIN;
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) {
+                                e[nb][r] = (kOwn ? acc[nb][r] * cq[nb] : acc[nb][r]) * sk[r] - m[nb];
+                                if (kEdge && !sees(pos[nb], window_lo(a, pos[nb]), a.sinks, t0 + 16 * u + 4 * lq + r)) e[nb][r] = -INFINITY;
+                                over = max(over, __float_as_int(e[nb][r]));  // positive floats order like their bits
+                            }
+                        if (__builtin_amdgcn_ballot_w64(over > 0) != 0) {
+                            bool open = false;
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+                                const float mx = fmaxf(fmaxf(e[nb][0], e[nb][1]), fmaxf(e[nb][2], e[nb][3]));  // relative to m
+                                float up = 0.0f;
+                                if (l[nb] == 0.0f) up = mx > -INFINITY ? mx + kOver : 0.0f;  // the column's first keys in this lane
+                                else if (mx > 0.0f) up = mx + kOver;
+                                l[nb] *= __builtin_amdgcn_exp2f(-up);
+                                m[nb] += up;
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) e[nb][r] -= up;
+                                open = open || (pos[nb] >= 0 && l[nb] == 0.0f && !(mx > -INFINITY));
+                            }
+                            force = __builtin_amdgcn_ballot_w64(open) != 0;
+                        }
+                        if (u < 3) product(u + 1);
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+                            l[nb] += (__builtin_amdgcn_exp2f(e[nb][0]) + __builtin_amdgcn_exp2f(e[nb][1])) +
+                                     (__builtin_amdgcn_exp2f(e[nb][2]) + __builtin_amdgcn_exp2f(e[nb][3]));
+                    }
+                };
+                if (edge) consume(std::true_type{});
+                else if (kOwn || force || !consume_fast()) consume(std::false_type{});
             }
+            if (nst < s_hi) commit(buf ^ 1);
+            __syncthreads();
+            st = nst;
         }
-        if (nst < s_hi) commit(buf ^ 1);
-        __syncthreads();
-        st = nst;
-    }
+    };
+    if (own) walk(std::true_type{});
+    else walk(std::false_type{});
     // ---- join the four lanes of a column; one (m, l) per column and chunk, or the finished statistic
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-        const float M = quad_max(m[nb]);
-        const float L = quad_sum(m[nb] == -INFINITY ? l[nb] : l[nb] * __builtin_amdgcn_exp2f(m[nb] - M));
-        const int c = wg_c0 + 16 * NB * wave + 16 * nb + li;
-        if (lq != 0 || c >= a.cols) continue;
+        const float mine = l[nb] == 0.0f ? -INFINITY : m[nb];
+        const float M = quad_max(mine);
+        const float L = quad_sum(l[nb] == 0.0f ? 0.0f : l[nb] * __builtin_amdgcn_exp2f(mine - M));
+        const int c = wv_c0 + 16 * nb + li;
+        if (lq != 0 || c >= a.lse_stride) continue;
         if (a.key_chunks == 1) {
-            a.lse[(int64_t)unit * a.cols + c] = L == 0.0f ? INFINITY : M + __builtin_amdgcn_logf(L);
-        } else {
+            a.lse[(int64_t)unit * a.lse_stride + c] = L == 0.0f ? INFINITY : M + __builtin_amdgcn_logf(L);
+        } else if (c < a.cols) {
             float *ml = a.part_ml + (((int64_t)unit * a.key_chunks + chunk) * a.cols + c) * 2;
             ml[0] = M;
             ml[1] = L;
@@ -237,12 +375,12 @@ __global__ __launch_bounds__(256, 2) void weights_stats_kernel(WeightsArgs a) {
 
 // lse of a column from its key chunks: sixteen columns a workgroup, the chunks of one over sixteen lanes.
 __global__ __launch_bounds__(256) void weights_join_kernel(WeightsArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15), n = (int64_t)a.B * a.Hkv * a.cols;
+    const int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x & 15), n = (int64_t)a.B * a.Hkv * a.lse_stride;
     const int part = threadIdx.x >> 4;
     __shared__ float sm_m[16][16], sm_l[16][16];
     float M = -INFINITY, L = 0.0f;
-    if (i < n) {
-        const int64_t unit = i / a.cols, c = i % a.cols;
+    const int64_t unit = i / a.lse_stride, c = i % a.lse_stride;
+    if (i < n && c < a.cols) {
         const float *ml = a.part_ml + (unit * a.key_chunks * a.cols + c) * 2;
         for (int k = part; k < a.key_chunks; k += 16) M = fmaxf(M, ml[(int64_t)k * a.cols * 2]);
         for (int k = part; k < a.key_chunks; k += 16) {
@@ -264,121 +402,166 @@ __global__ __launch_bounds__(256) void weights_join_kernel(WeightsArgs a) {
 }
 
 template <int D, bool FP8>
-__global__ __launch_bounds__(256, 2) void weights_columns_kernel(WeightsArgs a) {
+__global__ __launch_bounds__(kWThreads, 2) void weights_columns_kernel(WeightsArgs a) {
     constexpr int KG = D / 32, NU = D == 256 ? 2 : 4;  // 16-key tiles of a wavefront
-    constexpr int KEYS = 64 * NU;                      // keys of the workgroup
-    constexpr int CPR = D / 8, LOADS = kWStep * CPR / 256;  // 16-byte pieces of a column, pieces per thread and step
-    constexpr int SWZ = CPR < 16 ? CPR - 1 : 15;       // pieces are stored at piece ^ (column & SWZ): the sixteen columns a load reads lie in different banks
+    constexpr int KEYS = kWThreads / 4 * NU;                     // keys of the workgroup
+    constexpr int kCStep = D == 256 ? 64 : kCStepMax;
+    constexpr int CPR = D / 8, LOADS = kCStep * CPR / kWThreads;  // 16-byte pieces of a column, pieces per thread and step
+    constexpr int SWZ = CPR < 16 ? CPR - 1 : 15;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 15, lq = lane >> 4;
     const int units = a.B * a.Hkv;
+    // key blocks in ascending order: the first ones are seen by the most columns and start first
     const int unit = blockIdx.x % units, seg = (blockIdx.x / units) % a.segments, kb = blockIdx.x / units / a.segments;
     const int b = unit / a.Hkv, h = unit % a.Hkv;
     const int pos0 = first_pos(a, b), T = key_count(a, pos0);
     const int k0 = kb * KEYS, wk0 = k0 + 16 * NU * wave;
     if (k0 >= T) return;
-    const int per = a.segments == 1 ? (a.cols + kWStep - 1) / kWStep * kWStep : kWSegment;
-    int c_lo = seg * per, c_hi = min(a.cols, c_lo + per);
+    // steps of kCStep columns; this workgroup takes every a.segments-th of them
+    int c_lo = 0, c_hi = (a.cols + kCStep - 1) / kCStep * kCStep;
+    const int stride = kCStep * a.segments;
     // columns that can see a key of the block: from the query at its first key on; with a window, to the query that
     // loses its last key (unless the block holds sinks)
-    c_lo = max(c_lo, (int)(min((int64_t)a.cols, max((int64_t)0, ((int64_t)k0 - pos0) * a.G)) / kWStep * kWStep));
-    if (a.window && k0 >= a.sinks) c_hi = (int)min((int64_t)c_hi, max((int64_t)0, ((int64_t)k0 + KEYS - 1 + a.window - pos0) * a.G));
-    __shared__ __attribute__((aligned(16))) uint8_t sm_q[2][kWStep * D * 2];
-    __shared__ float sm_lse[2][kWStep];
+    c_lo = max(c_lo, (int)(min((int64_t)a.cols, max((int64_t)0, ((int64_t)k0 - pos0) * a.G)) / kCStep * kCStep));
+    c_lo += (seg + a.segments - c_lo / kCStep % a.segments) % a.segments * kCStep;
+    if (a.window && k0 >= a.sinks)
+        c_hi = (int)min((int64_t)c_hi, (max((int64_t)0, ((int64_t)k0 + KEYS - 1 + a.window - pos0) * a.G) + kCStep - 1) / kCStep * kCStep);
+    // two buffers of kCStep columns as they lie in q (16-byte piece pc of a column at piece pc ^ (column & SWZ): the sixteen
+    // columns a load of operands reads lie in different banks), and their lse.  The copies go straight from memory to LDS.
+    constexpr int kTileBytes = kCStep * D * 2, kTile = kTileBytes + kCStep * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t sm[2 * kTile];
 
-    float4v sum[NU];
+    float4v sum[NU], before[NU];  // `before`: what the weights of this lane's keys start from, loaded while there is other work
 #pragma unroll
-    for (int u = 0; u < NU; ++u) sum[u] = (float4v){0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < NU; ++u) {
+        sum[u] = before[u] = (float4v){0.f, 0.f, 0.f, 0.f};
+        if (a.segments == 1 && a.in && li == 0) before[u] = *(const float4v *)(a.in + (int64_t)unit * a.stride + min(wk0 + 16 * u + 4 * lq, (int)a.stride - 4));
+    }
     if (c_lo < c_hi) {
+        // ---- columns, kCStep a step: copy i of this thread is piece (x % CPR) of the tile's column x / CPR, x = tid + 512 i.
+        //      Where kCStep is a multiple of G the columns' rows move by one constant from step to step.
+        const float *lse = a.lse + (int64_t)unit * a.lse_stride;
+        const uint8_t *qb = (const uint8_t *)(a.q + ((int64_t)b * a.S * a.Hq + h * a.G) * D);
+        const bool regular = kCStep % a.G == 0;
+        const int64_t step_bytes = (int64_t)(kCStep / a.G) * a.Hq * D * 2;
+        uint32_t off[LOADS];
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            const int x = tid + kWThreads * i, c = x / CPR;
+            off[i] = (uint32_t)(((c / a.G) * a.Hq + c % a.G) * D * 2 + 16 * ((x % CPR) ^ (c & SWZ)));
+        }
+        auto fetch = [&](int c0, int buf) {
+            uint8_t *dst = sm + buf * kTile + 1024 * wave;
+            if (regular && c0 + kCStep <= a.cols) {
+                const uint8_t *src = qb + (int64_t)(c0 / kCStep) * step_bytes;
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) copy16_to_lds(src + off[i], dst + 16 * kWThreads * i);
+            } else {  // any other group size; the last, partial step repeats the last column
+#pragma unroll
+                for (int i = 0; i < LOADS; ++i) {
+                    const int x = tid + kWThreads * i, c = x / CPR, cc = min(c0 + c, a.cols - 1);
+                    const uint8_t *src = qb + ((int64_t)(cc / a.G) * a.Hq + cc % a.G) * (D * 2) + 16 * ((x % CPR) ^ (c & SWZ));
+                    copy16_to_lds(src, dst + 16 * kWThreads * i);
+                }
+            }
+            if (wave < kCStep / 64) copy4_to_lds(lse + c0 + 64 * wave + lane, sm + buf * kTile + kTileBytes + 256 * wave);
+        };
         // ---- keys: lane (li, lq) holds key 16u + li, d = 32j + 8 lq + e, as bf16
         bf16x8 kop[NU][KG];
         float4v sk[NU];  // scale of keys 16u + 4 lq + r, times the softmax scale in log2 units
+        {
+            const KeyBase k = key_base(a, b, h, min(wk0, T - 1), D, FP8);  // (a wavefront behind the last key: any address)
+            const int last = max(0, T - 1 - wk0);
+            u32x2 w[NU][KG];
 #pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            int64_t ku;
-            int slot;
-            resolve(a.ka, b, min(wk0 + 16 * u + li, T - 1), ku, slot);
-            const uint8_t *src = a.kc + ku * a.ka.code_stride_seq + (int64_t)h * a.ka.code_stride_head + (int64_t)slot * D + 8 * lq;
+            for (int u = 0; u < NU; ++u) {
+                const uint8_t *src = k.codes + (uint32_t)(min(16 * u + li, last) * D + 8 * lq);
 #pragma unroll
-            for (int j = 0; j < KG; ++j) {
-                const u32x2 w = *(const u32x2 *)(src + 32 * j);
-                uint32_t o[4];
+                for (int j = 0; j < KG; ++j) w[u][j] = *(const u32x2 *)(src + 32 * j);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint32_t x = w[e >> 1] >> (16 * (e & 1));
-                    o[e] = code_to_bf16(x & 0xffu, FP8) | (code_to_bf16((x >> 8) & 0xffu, FP8) << 16);
-                }
-                kop[u][j] = pack_bf16x8(o[0], o[1], o[2], o[3]);
+                for (int r = 0; r < 4; ++r) sk[u][r] = a.scale_log2e * (FP8 ? a.ks[(int64_t)b * a.Hkv + h] : k.scales[min(16 * u + 4 * lq + r, last)]);
             }
+            fetch(c_lo, 0);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                float s;
-                if (FP8) s = a.ks[(int64_t)b * a.Hkv + h];
-                else {
-                    resolve(a.ka, b, min(wk0 + 16 * u + 4 * lq + r, T - 1), ku, slot);
-                    s = a.ks[ku * a.ka.scale_stride_seq + (int64_t)h * a.ka.scale_stride_head + slot];
-                }
-                sk[u][r] = s * a.scale_log2e;
-            }
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int j = 0; j < KG; ++j) kop[u][j] = codes_to_bf16<FP8>(w[u][j][0], w[u][j][1]);
         }
-        u32x4 raw[LOADS];
-        float rawl = 0.0f;
-        const float *lse = a.lse + (int64_t)unit * a.cols;
-        auto load = [&](int c0) {
+        // one step of a wavefront; kEdge: some (key, column) pair may be hidden
+        uint32_t qoff[KG];  // this lane's piece of the operand of d-group j, column li
 #pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int x = tid + 256 * i, c = min(c0 + x / CPR, a.cols - 1);
-                const int s = c / a.G, g = c % a.G;
-                raw[i] = *(const u32x4 *)(a.q + (((int64_t)b * a.S + s) * a.Hq + h * a.G + g) * D + 8 * (x % CPR));
-            }
-            if (tid < kWStep) rawl = c0 + tid < c_hi ? lse[c0 + tid] : INFINITY;  // +inf: no weight
-        };
-        auto commit = [&](int buf) {
-#pragma unroll
-            for (int i = 0; i < LOADS; ++i) {
-                const int x = tid + 256 * i, c = x / CPR, pc = x % CPR;
-                *(u32x4 *)(sm_q[buf] + (c * CPR + (pc ^ (c & SWZ))) * 16) = raw[i];
-            }
-            if (tid < kWStep) sm_lse[buf][tid] = rawl;
-        };
-        load(c_lo);
-        commit(0);
-        __syncthreads();
-        int buf = 0;
-        for (int c0 = c_lo; c0 < c_hi; c0 += kWStep, buf ^= 1) {
-            if (c0 + kWStep < c_hi) load(c0 + kWStep);
-            const int p0 = pos0 + c0 / a.G, p1 = pos0 + min(c0 + kWStep - 1, a.cols - 1) / a.G;
-            if (wk0 <= p1 && wk0 < T) {
-                // some (key, column) pair of the step may be hidden: in the future, out of the window, past the last key or in no sequence
-                const bool edge = wk0 + 16 * NU - 1 > p0 || wk0 + 16 * NU > T || p0 < 0 || p1 >= a.max_seq_len || (a.window && wk0 <= p1 - a.window);
-#pragma unroll
-                for (int nb = 0; nb < 4; ++nb) {
-                    const int c = 16 * nb + li;
-                    bf16x8 qop[KG];
-#pragma unroll
-                    for (int j = 0; j < KG; ++j) qop[j] = *(const bf16x8 *)(sm_q[buf] + (c * CPR + ((4 * j + lq) ^ (c & SWZ))) * 16);
-                    const float ref = sm_lse[buf][c];
-                    int p = -1;
-                    if (edge) {
-                        p = pos0 + (c0 + c) / a.G;
-                        if (p >= a.max_seq_len) p = -1;
-                    }
-#pragma unroll
-                    for (int u = 0; u < NU; ++u) {
-                        float4v acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int j = 0; j < KG; ++j) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop[u][j], qop[j], acc, 0, 0, 0);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            float w = __builtin_amdgcn_exp2f(acc[r] * sk[u][r] - ref);
-                            if (edge && !(sees(a, p, wk0 + 16 * u + 4 * lq + r) && wk0 + 16 * u + 4 * lq + r < T)) w = 0.0f;
-                            sum[u][r] += w;
-                        }
-                    }
+        for (int j = 0; j < KG; ++j) qoff[j] = (uint32_t)((li * CPR + ((4 * j + lq) ^ (li & SWZ))) * 16);
+        auto consume = [&](auto buf_tag, int c0, auto edge_tag) {
+            constexpr int kBuf = decltype(buf_tag)::value;
+            constexpr bool kEdge = decltype(edge_tag)::value;
+            const uint8_t *tile = sm + kBuf * kTile;
+            // Operand block k = KG nb + j is read kAhead blocks ahead of its products through a ring of registers; the
+            // weights of the previous sixteen columns are made among the products of these, four NU of them spread over
+            // KG NU products.  The order is pinned: left to itself the compiler reads each operand right before its use.
+            constexpr int kBlocks = kCStep / 16 * KG, kAhead = 4, kRing = 8;
+            float4v acc[2][NU];
+            bf16x8 ring[kRing];
+            float ref[2] = {0.0f, 0.0f}, pend = 0.0f;
+            int p = -1, lo = 0;
+            auto read = [&](int k) { return *(const bf16x8 *)(tile + (k / KG) * 16 * CPR * 16 + qoff[k % KG]); };
+            auto add = [&](int e) {  // weight e of a group of sixteen columns: tile e / 4, key row e % 4
+                if constexpr (kEdge) sum[e >> 2][e & 3] += sees(p, lo, a.sinks, wk0 + 16 * (e >> 2) + 4 * lq + (e & 3)) ? pend : 0.0f;
+                else sum[e >> 2][e & 3] += pend;
+            };
+            auto weight = [&](int nb, int e) {
+                if (e > 0) add(e - 1);
+                pend = __builtin_amdgcn_exp2f(acc[nb & 1][e >> 2][e & 3] * sk[e >> 2][e & 3] - ref[nb & 1]);
+            };
+            auto bounds = [&](int nb) {
+                if constexpr (kEdge) {
+                    p = pos0 + (c0 + 16 * nb + li) / a.G;
+                    if (p >= a.max_seq_len) p = -1;
+                    lo = window_lo(a, p);
+                    p = min(p, T - 1);
                 }
+            };
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) ring[k] = read(k);
+#pragma unroll
+            for (int k = 0; k < kBlocks; ++k) {
+                const int nb = k / KG, j = k % KG;
+                if (k + kAhead < kBlocks) ring[(k + kAhead) % kRing] = read(k + kAhead);
+                if (j == 0) ref[nb & 1] = ((const float *)(tile + kTileBytes))[16 * nb + li];
+                if (j == 0 && nb > 0) bounds(nb - 1);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int u = 0; u < NU; ++u) {
+                    acc[nb & 1][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop[u][j], ring[k % kRing], j == 0 ? (float4v){0.f, 0.f, 0.f, 0.f} : acc[nb & 1][u], 0, 0, 0);
+                    if (nb > 0) {
+                        const int i = j * NU + u;  // product i of KG NU
+#pragma unroll
+                        for (int e = i * 4 / KG; e < (i + 1) * 4 / KG; ++e) weight(nb - 1, e);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (nb > 0 && j == KG - 1) add(4 * NU - 1);
             }
-            if (c0 + kWStep < c_hi) commit(buf ^ 1);
+            bounds(kCStep / 16 - 1);
+#pragma unroll
+            for (int e = 0; e < 4 * NU; ++e) weight(kCStep / 16 - 1, e);
+            add(4 * NU - 1);
+        };
+        auto step = [&](auto buf_tag, int c0) {
+            // this wavefront's copies of the tile have landed, then everybody's; nobody reads the other buffer any more
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
+            if (c0 + stride < c_hi) fetch(c0 + stride, 1 - decltype(buf_tag)::value);
+            const int p0 = pos0 + c0 / a.G, p1 = pos0 + min(c0 + kCStep - 1, a.cols - 1) / a.G;
+            if (wk0 <= p1 && wk0 < T) {
+                // hidden: in the future, out of the window, past the last key or in no sequence
+                const bool edge = wk0 + 16 * NU - 1 > p0 || wk0 + 16 * NU > T || p0 < 0 || p1 >= a.max_seq_len || (a.window && wk0 <= p1 - a.window);
+                if (edge) consume(buf_tag, c0, std::true_type{});
+                else consume(buf_tag, c0, std::false_type{});
+            }
+        };
+        for (int c0 = c_lo; c0 < c_hi; c0 += 2 * stride) {
+            step(std::integral_constant<int, 0>{}, c0);
+            if (c0 + stride < c_hi) step(std::integral_constant<int, 1>{}, c0 + stride);
         }
     }
     // ---- the sixteen columns of a key's lanes meet; lane li = 0 of each group writes its four keys
@@ -386,12 +569,7 @@ __global__ __launch_bounds__(256, 2) void weights_columns_kernel(WeightsArgs a) 
     for (int u = 0; u < NU; ++u) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            float x = sum[u][r];
-            x += __shfl_xor(x, 1, 64);
-            x += __shfl_xor(x, 2, 64);
-            x += __shfl_xor(x, 4, 64);
-            x += __shfl_xor(x, 8, 64);
-            sum[u][r] = x;
+            sum[u][r] = row_sum(sum[u][r]);
         }
         const int t = wk0 + 16 * u + 4 * lq;
         if (li != 0 || t >= T) continue;
@@ -399,7 +577,7 @@ __global__ __launch_bounds__(256, 2) void weights_columns_kernel(WeightsArgs a) 
             const int64_t o = (int64_t)unit * a.stride + t;
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                if (t + r < T) a.out[o + r] = (a.in ? a.in[o + r] : 0.0f) + sum[u][r];
+                if (t + r < T) a.out[o + r] = before[u][r] + sum[u][r];
         } else {
             *(float4v *)(a.part_w + ((int64_t)seg * units + unit) * a.part_stride + t) = sum[u];
         }
@@ -424,7 +602,8 @@ int validate_layout(const hs_kv_layout *l, int B, int S, int Hkv, int D, bool ne
 int check_weights(const float *in, const float *out, int64_t stride, int max_seq_len, bool used);
 
 struct WeightsPlan {
-    int64_t cols, col_blocks, key_blocks;
+    int64_t cols, col_blocks, key_blocks, lse_stride;
+    int nb;  // 16-column blocks per wavefront of the first kernel
     int key_chunks, chunk_tokens, segments;
     int64_t part_stride;
     size_t ml_floats, lse_floats, w_floats;
@@ -434,20 +613,26 @@ static WeightsPlan plan_weights(int B, int S, int Hq, int Hkv, int D, int max_se
     WeightsPlan p;
     const int64_t units = (int64_t)B * Hkv;
     p.cols = (int64_t)S * (Hq / Hkv);
-    const int wg_cols = D == 256 ? 128 : 256, wg_keys = D == 256 ? 128 : 256;
+    // a wavefront holds 32 columns; sixteen at head_dim 256 (registers) and when all columns fit one workgroup that way
+    p.nb = p.cols <= 64 ? 1 : p.cols <= 128 || D == 256 ? 2 : 4;
+    const int wg_cols = kWThreads / 4 * p.nb, wg_keys = kWThreads / 4 * (D == 256 ? 2 : 4);
     p.col_blocks = (p.cols + wg_cols - 1) / wg_cols;
     p.key_blocks = ((int64_t)max_seq_len + wg_keys - 1) / wg_keys;
     // First kernel: few columns (an observation window) leave most CUs idle unless the keys are split, into chunks of
     // at least 512.
-    const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(1, units * p.col_blocks));
+    const int64_t want = std::max<int64_t>(1, CHN / std::max<int64_t>(1, units * p.col_blocks));
     int64_t ct = ((int64_t)max_seq_len + want - 1) / want;
-    ct = std::max<int64_t>(512, (ct + kWStep - 1) / kWStep * kWStep);
+    ct = std::max<int64_t>(CHM, (ct + kWStep - 1) / kWStep * kWStep);
     p.chunk_tokens = (int)std::min<int64_t>(ct, ((int64_t)max_seq_len + kWStep - 1) / kWStep * kWStep);
     p.key_chunks = (int)(((int64_t)max_seq_len + p.chunk_tokens - 1) / p.chunk_tokens);
-    // Second kernel: the columns of a key block in segments, which also evens out the causal triangle.
-    p.segments = (int)((p.cols + kWSegment - 1) / kWSegment);
+    // Second kernel: two workgroups are resident on each of 256 CUs, and each of them should come round twice: started in
+    // order of their work, long items then meet short ones and the causal triangle evens out (4 x 4096 tokens, 16 key
+    // blocks on 32 units, us: @1 one share of the columns, @2 two, @4 four).
+    const int64_t items = units * p.key_blocks, steps = (p.cols + kCStepMax - 1) / kCStepMax;
+    p.segments = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(steps, 16), (1024 + items - 1) / items));
     p.part_stride = p.key_blocks * wg_keys;
-    p.lse_floats = (size_t)(units * p.cols + 3) / 4 * 4;
+    p.lse_stride = (p.cols + 127) / 128 * 128;
+    p.lse_floats = (size_t)(units * p.lse_stride);
     p.ml_floats = p.key_chunks > 1 ? (size_t)units * p.key_chunks * p.cols * 2 : 0;
     p.w_floats = p.segments > 1 ? (size_t)p.segments * units * p.part_stride : 0;
     return p;
@@ -456,9 +641,12 @@ static WeightsPlan plan_weights(int B, int S, int Hq, int Hkv, int D, int max_se
 template <int D, bool FP8>
 static void launch_weights(const WeightsArgs &a, const WeightsPlan &p, hipStream_t st) {
     const int64_t units = (int64_t)a.B * a.Hkv;
-    weights_stats_kernel<D, FP8><<<(unsigned)(units * p.key_chunks * p.col_blocks), 256, 0, st>>>(a);
-    if (p.key_chunks > 1) weights_join_kernel<<<(unsigned)((units * p.cols + 15) / 16), 256, 0, st>>>(a);
-    weights_columns_kernel<D, FP8><<<(unsigned)(units * p.segments * p.key_blocks), 256, 0, st>>>(a);
+    const unsigned grid = (unsigned)(units * p.key_chunks * p.col_blocks);
+    if (p.nb == 1) weights_stats_kernel<D, FP8, 1><<<grid, kWThreads, 0, st>>>(a);
+    else if (p.nb == 2) weights_stats_kernel<D, FP8, 2><<<grid, kWThreads, 0, st>>>(a);
+    else if constexpr (D < 256) weights_stats_kernel<D, FP8, 4><<<grid, kWThreads, 0, st>>>(a);
+    if (p.key_chunks > 1) weights_join_kernel<<<(unsigned)((units * p.lse_stride + 15) / 16), 256, 0, st>>>(a);
+    weights_columns_kernel<D, FP8><<<(unsigned)(units * p.segments * p.key_blocks), kWThreads, 0, st>>>(a);
     if (p.segments > 1) weights_sum_kernel<<<dim3((unsigned)((a.max_seq_len + 1023) / 1024), (unsigned)units), 256, 0, st>>>(a);
 }
 
@@ -483,6 +671,8 @@ int hs_attn_weights(int fmt_fp8, const void *q, const void *k_codes, const float
     if (max_seq_len <= 0) return fail(HS_ERR_INVALID_ARGUMENT, "max_seq_len must be positive");
     if (layout->prefill_window < 0 || layout->attn_sinks < 0)
         return fail(HS_ERR_INVALID_ARGUMENT, "negative prefill_window %d or attn_sinks %d", layout->prefill_window, layout->attn_sinks);
+    if (layout->k_block_table && (layout->capacity_tokens % kWStep) != 0)  // a step reads 64 tokens of one block
+        return fail(HS_ERR_INVALID_ARGUMENT, "paged blocks must hold a multiple of %d tokens", kWStep);
     const int64_t cap = layout->k_block_table ? (int64_t)layout->capacity_tokens * layout->block_table_stride : layout->capacity_tokens;
     if (max_seq_len > cap)
         return fail(HS_ERR_OVERFLOW, "max_seq_len %d exceeds what the cache can hold (%lld tokens)", max_seq_len, (long long)cap);
@@ -515,7 +705,7 @@ int hs_attn_weights(int fmt_fp8, const void *q, const void *k_codes, const float
     a.part_ml = a.part_w + p.w_floats;
     a.part_stride = p.part_stride;
     a.start_pos = start_pos; a.B = B; a.S = S; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv;
-    a.cols = (int)p.cols; a.max_seq_len = max_seq_len;
+    a.cols = (int)p.cols; a.lse_stride = (int)p.lse_stride; a.max_seq_len = max_seq_len;
     a.window = layout->prefill_window; a.sinks = std::min(layout->attn_sinks, max_seq_len);
     a.key_chunks = p.key_chunks; a.chunk_tokens = p.chunk_tokens; a.segments = p.segments;
     a.scale_log2e = softmax_scale * kWLog2e;

@@ -53,25 +53,26 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 #undef HS_DPP_ADD
     return v;
 }
-// One workgroup per row.  A thread owns four neighbouring weights of every 4 THREADS and keeps the keys of 4 NV of them in
-// registers, so a row of up to 4 NV THREADS tokens is read once, all loads in flight together, and the passes run on
-// registers; a longer row is read again for every pass, a tile of that length at a time.  Protected tokens take the
-// largest key, so every pass is one comparison per token.  What a row costs is the latency of its steps (three
-// histograms with a scan each, one scan for the list), so the scans run on the vector pipe and few waves take part in
-// a barrier: four for rows of up to 8192 tokens, sixteen beyond.
-constexpr int kSelectNV = 8;
+// One workgroup per row.  The weights' keys go to LDS once (protected tokens take the largest key, so every pass is one
+// comparison per token) and all passes read them there; a row longer than kTile tokens is read again for every pass, a
+// tile at a time.  A row is a chain of short steps -- three histograms with a scan each, one scan for the list -- so what
+// it costs is latency: the scans run on the vector pipe, a pass counts without branches (what it
+// does not count goes to a place of the lane's own), and sixteen wavefronts hide each other's latencies (with four per
+// row and 32 weights a thread: 25 us at 64 x 8 rows of 8192 tokens against @).
 constexpr uint32_t kProtected = 0xffffffffu, kZeroKey = 0x80000000u;
-template <int THREADS>
-__global__ __launch_bounds__(THREADS, 4) void evict_select_kernel(EvictArgs a) {
-    constexpr int NV = kSelectNV, kWaves = THREADS / 64, kTile = NV * 4 * THREADS, BPT = 2048 / THREADS, kCounts = NV * kWaves;
+template <int TILE>
+__global__ __launch_bounds__(1024) void evict_select_kernel(EvictArgs a) {
+    constexpr int THREADS = 1024;
+    constexpr uint32_t kCand = 1024;
+    constexpr int kWaves = THREADS / 64, kGroup = 4 * THREADS, kGroups = TILE / kGroup, kCounts = kGroups * kWaves;
     static_assert(kCounts <= 128, "two counts per lane");
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int64_t row = (int64_t)b * a.Hkv + h;
     const int L = min(max(a.seq_lens[b], 0), a.max_seq_len);
     const float *w = a.w ? a.w + row * a.w_stride : nullptr;
     int32_t *list = a.list + row * a.budget;
-    __shared__ __attribute__((aligned(16))) uint32_t sm_hist[3][2048];
-    __shared__ uint32_t sm_wave[kWaves], sm_pick[3][2], sm_cnt[kCounts];
+    __shared__ __attribute__((aligned(16))) uint32_t sm_key[TILE], sm_hist[2048 + 64];  // bins, and a place per lane for what is not counted
+    __shared__ uint32_t sm_list[kCand], sm_wave[4], sm_pick[3], sm_cand, sm_cnt[kCounts], sm_pre[kCounts + 1];
     __shared__ int sm_first;
     const int n = min(L, a.budget);
     if (L <= a.budget || w == nullptr) {
@@ -81,143 +82,161 @@ __global__ __launch_bounds__(THREADS, 4) void evict_select_kernel(EvictArgs a) {
         if (tid == 0) sm_first = s;
     } else {
         const int lo = a.sinks, hi = L - a.recent, K = a.budget - a.sinks - a.recent;
-        const int tiles = (L + kTile - 1) / kTile;
-        float4v x[NV];
-        uint32_t key[NV][4];  // tokens behind the row take key 0: the lowest one, and last among its equals
-        auto load = [&](int tile) {
+        const int tiles = (L + TILE - 1) / TILE;
+        // keys of the tile that starts at `base`: every thread reads back only what it wrote.  Tokens behind the row
+        // take key 0: the lowest one, and last among its equals.
+        auto load = [&](int base) {
+            float4v x[kGroups];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int t0 = tile * kTile + 4 * (i * THREADS + tid);
-                x[i] = t0 < L ? *(const float4v *)(w + t0) : (float4v){0.f, 0.f, 0.f, 0.f};  // rows are a multiple of four long
+            for (int i = 0; i < kGroups; ++i) {
+                const int t = base + i * kGroup + 4 * tid;
+                x[i] = t < L ? *(const float4v *)(w + t) : (float4v){0.f, 0.f, 0.f, 0.f};  // rows are a multiple of four long
             }
-        };
-        auto make_keys = [&](int tile) {
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int t0 = tile * kTile + 4 * (i * THREADS + tid);
+            for (int i = 0; i < kGroups; ++i) {
+                u32x4 k;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int t = t0 + e;
-                    key[i][e] = t >= L ? 0u : t < lo || t >= hi ? kProtected : weight_key(x[i][e]);
+                    const int t = base + i * kGroup + 4 * tid + e;
+                    k[e] = t >= L ? 0u : t < lo || t >= hi ? kProtected : weight_key(x[i][e]);
                 }
+                *(u32x4 *)&sm_key[i * kGroup + 4 * tid] = k;
             }
         };
-        // groups of four tokens per thread that lie in the row (uniform over the workgroup)
-        auto groups = [&](int tile) { return min(NV, (L - tile * kTile + 4 * THREADS - 1) / (4 * THREADS)); };
-        load(0);
-        for (int i = tid; i < 3 * 2048 / 4; i += THREADS) ((u32x4 *)&sm_hist[0][0])[i] = (u32x4){0u, 0u, 0u, 0u};
         if (tid == 0) sm_first = n;
-        __syncthreads();
-        make_keys(0);
+        load(0);
         // ---- key of the K-th heaviest token of [lo, hi), three digits of 11, 11 and 10 bits; `need` of those that share
-        //      it stay, the lowest positions first
-        uint32_t prefix = kProtected - 1, need = 0;
-        if (K > 0) {
-            constexpr int shift[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
-            constexpr uint32_t mask[3] = {2047u, 2047u, 1023u};
-            prefix = 0;
-            need = (uint32_t)K;
-#pragma unroll
-            for (int p = 0; p < 3; ++p) {
+        //      it stay, the lowest positions first.  The keys that share the first digit are few as a rule: they are put
+        //      together and the other digits found among them, unless they are more than kCand.
+        uint32_t prefix = K > 0 ? 0u : kProtected - 1, need = (uint32_t)K, cand = kCand + 1;
+#pragma unroll 1
+        for (int shift = 21; K > 0; shift = shift == 21 ? 10 : 0) {
+            const uint32_t mask = shift == 0 ? 1023u : 2047u, fixed = shift == 21 ? 0u : shift == 10 ? 0xffe00000u : 0xfffffc00u;
+            if (tid < 512) *(u32x4 *)&sm_hist[4 * tid] = (u32x4){0u, 0u, 0u, 0u};
+            if (tid == 0) sm_cand = 0;
+            __syncthreads();
+            if (cand <= kCand) {
+                for (uint32_t i = tid; i < cand; i += THREADS) {
+                    const uint32_t k = sm_list[i];
+                    if (((k ^ prefix) & fixed) == 0u) atomicAdd(&sm_hist[(k >> shift) & mask], 1u);
+                }
+            } else {
                 uint32_t zeros = 0;  // tokens without any weight are many and would queue at one counter
+#pragma unroll 1
                 for (int tile = 0; tile < tiles; ++tile) {
-                    if (tiles > 1) {
-                        load(tile);
-                        make_keys(tile);
-                    }
-                    const int ng = groups(tile);
+                    if (tiles > 1) load(tile * TILE);
+                    const int left = L - tile * TILE - 4 * tid;  // tokens of the row from this thread's first one on
 #pragma unroll
-                    for (int i = 0; i < NV; ++i) {
-                        if (i >= ng) break;
+                    for (int i = 0; i < kGroups; ++i) {
+                        if (i * kGroup >= left) break;
+                        const u32x4 k = *(const u32x4 *)&sm_key[i * kGroup + 4 * tid];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const uint32_t k = key[i][e];
-                            if (p == 0 && k == kZeroKey) ++zeros;
-                            else if (k != kProtected && (p == 0 || ((k ^ prefix) >> (shift[p] + bits[p])) == 0u))
-                                atomicAdd(&sm_hist[p][(k >> shift[p]) & mask[p]], 1u);
+                            const bool none = k[e] == kZeroKey && shift == 21;
+                            const bool counts = k[e] != kProtected && ((k[e] ^ prefix) & fixed) == 0u && !none && i * kGroup + e < left;
+                            zeros += none ? 1u : 0u;
+                            atomicAdd(&sm_hist[counts ? (k[e] >> shift) & mask : 2048u + lane], 1u);
                         }
                     }
                 }
-                if (p == 0) {
-                    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(zeros), 63);
-                    if (lane == 0 && all != 0) atomicAdd(&sm_hist[0][kZeroKey >> 21], all);
+                if (shift == 21) {
+                    zeros = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(zeros), 63);
+                    if (lane == 0 && zeros != 0) atomicAdd(&sm_hist[kZeroKey >> 21], zeros);
                 }
-                __syncthreads();
-                // the digit at which the count from the top reaches `need`: thread i owns the BPT bins below 2048 - BPT i
-                uint32_t bin[BPT], sum = 0;
+            }
+            __syncthreads();
+            // the digit at which the count from the top reaches `need`: eight bins for each thread of the first four
+            // wavefronts, thread i those below 2048 - 8 i
+            uint32_t bin[8], sum = 0, incl = 0;
+            if (wave < 4) {
+                const u32x4 b0 = *(const u32x4 *)&sm_hist[2040 - 8 * tid], b1 = *(const u32x4 *)&sm_hist[2044 - 8 * tid];
 #pragma unroll
-                for (int e = 0; e < BPT; ++e) bin[e] = sm_hist[p][2048 - BPT * (tid + 1) + e];
-#pragma unroll
-                for (int e = 0; e < BPT; ++e) sum += bin[e];
-                uint32_t incl = wave_scan(sum);
+                for (int e = 0; e < 4; ++e) {
+                    bin[e] = b0[e];
+                    bin[4 + e] = b1[e];
+                    sum += b0[e] + b1[e];
+                }
+                incl = wave_scan(sum);
                 if (lane == 63) sm_wave[wave] = incl;
-                __syncthreads();
-                const uint32_t totals = wave_scan(lane < kWaves ? sm_wave[lane] : 0u);
-                if (wave > 0) incl += (uint32_t)__builtin_amdgcn_readlane((int)totals, wave - 1);
+            }
+            __syncthreads();
+            if (wave < 4) {
+                for (int v = 0; v < wave; ++v) incl += sm_wave[v];
                 uint32_t excl = incl - sum;
                 if (excl < need && need <= incl) {
 #pragma unroll
-                    for (int e = BPT - 1; e >= 0; --e) {
+                    for (int e = 7; e >= 0; --e) {
                         if (excl < need && need <= excl + bin[e]) {
-                            sm_pick[p][0] = (uint32_t)(2048 - BPT * (tid + 1) + e);
-                            sm_pick[p][1] = need - excl;
+                            sm_pick[0] = (uint32_t)(2040 - 8 * tid + e);
+                            sm_pick[1] = need - excl;
+                            sm_pick[2] = bin[e];
                         }
                         excl += bin[e];
                     }
                 }
+            }
+            __syncthreads();
+            prefix |= sm_pick[0] << shift;
+            need = sm_pick[1];
+            if (shift == 0) break;
+            if (shift == 21 && tiles == 1 && sm_pick[2] <= kCand) {
+                cand = sm_pick[2];
+                const int left = L - 4 * tid;
+#pragma unroll
+                for (int i = 0; i < kGroups; ++i) {
+                    if (i * kGroup >= left) break;
+                    const u32x4 k = *(const u32x4 *)&sm_key[i * kGroup + 4 * tid];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if ((k[e] ^ prefix) < (1u << 21) && k[e] != kProtected && i * kGroup + e < left) sm_list[atomicAdd(&sm_cand, 1u)] = k[e];
+                }
                 __syncthreads();
-                prefix |= sm_pick[p][0] << shift[p];
-                need = sm_pick[p][1];
             }
         }
         // ---- list, in order.  A token stays if its key is larger, or one of the first `need` equal ones.
         //      Counts travel in pairs: larger ones in the low half, ties in the high one (a tile holds at most 32768).
-        float *wo = a.w == a.wo ? a.wo + row * a.wo_stride : nullptr;  // in place; otherwise they move with their tokens
         uint32_t sure = 0, ties = 0;  // of the tiles before this one
+#pragma unroll 1
         for (int tile = 0; tile < tiles; ++tile) {
-            if (tiles > 1) {
-                load(tile);
-                make_keys(tile);
-            }
-            const int ng = groups(tile);
-            uint32_t below[NV];
+            if (tiles > 1) load(tile * TILE);
+            const int base = tile * TILE, groups = (min(TILE, L - base) + kGroup - 1) / kGroup;
+            auto pairs = [&](const u32x4 &k) {
+                uint32_t c = 0;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                uint32_t cnt = 0;
-                if (i < ng) {
+                for (int e = 0; e < 4; ++e) c += k[e] > prefix ? 1u : k[e] == prefix ? 0x10000u : 0u;
+                return c;
+            };
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) cnt += key[i][e] > prefix ? 1u : key[i][e] == prefix ? 0x10000u : 0u;
-                }
-                const uint32_t incl = wave_scan(cnt);
+            for (int i = 0; i < kGroups; ++i) {
+                if (i >= groups) break;
+                const uint32_t incl = wave_scan(pairs(*(const u32x4 *)&sm_key[i * kGroup + 4 * tid]));
                 if (lane == 63) sm_cnt[i * kWaves + wave] = incl;
-                below[i] = incl - cnt;
             }
             __syncthreads();
-            // counts in the order of the tokens: entry i * kWaves + wave.  Every wavefront sums them up for itself.
-            uint32_t c0 = 0, c1 = 0;
-            if (2 * lane < kCounts) {
-                c0 = sm_cnt[2 * lane];
-                c1 = sm_cnt[2 * lane + 1];
+            // counts in the order of the tokens: entry i * kWaves + wave; the first wavefront sums them up
+            if (wave == 0) {
+                const uint32_t c0 = 2 * lane < groups * kWaves ? sm_cnt[2 * lane] : 0u, c1 = 2 * lane + 1 < groups * kWaves ? sm_cnt[2 * lane + 1] : 0u;
+                const uint32_t incl = wave_scan(c0 + c1);
+                if (2 * lane < kCounts) {
+                    sm_pre[2 * lane + 1] = incl - c1;
+                    sm_pre[2 * lane + 2] = incl;
+                }
+                if (lane == 0) sm_pre[0] = 0;
             }
-            const uint32_t pair = wave_scan(c0 + c1);
-            __syncthreads();  // sm_cnt may be written again; with weights in place: this tile has been read everywhere
+            __syncthreads();
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                if (i >= ng) break;
-                const int at = i * kWaves + wave;
-                uint32_t before = (uint32_t)__builtin_amdgcn_readlane((int)pair, at >> 1) - (uint32_t)__builtin_amdgcn_readlane((int)c1, at >> 1);
-                if (!(at & 1)) before -= (uint32_t)__builtin_amdgcn_readlane((int)c0, at >> 1);
-                before += below[i];
+            for (int i = 0; i < kGroups; ++i) {
+                if (i >= groups) break;
+                const int g = i * kGroup + 4 * tid;
+                const u32x4 k = *(const u32x4 *)&sm_key[g];
+                const uint32_t cnt = pairs(k), before = sm_pre[i * kWaves + wave] + wave_scan(cnt) - cnt;
                 uint32_t s = sure + (before & 0xffffu), q = ties + (before >> 16);
-                const int t0 = tile * kTile + 4 * (i * THREADS + tid);
                 bool gap = false;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const bool is_sure = key[i][e] > prefix, is_tie = key[i][e] == prefix;
+                    const bool is_sure = k[e] > prefix, is_tie = k[e] == prefix;
                     if (is_sure || (is_tie && q < need)) {
-                        const int r = (int)(s + min(q, need));
-                        list[r] = t0 + e;
-                        if (wo) wo[r] = x[i][e];  // r <= t, and this tile has been read
+                        list[s + min(q, need)] = base + g + e;
                     } else {
                         gap = true;
                     }
@@ -226,17 +245,28 @@ __global__ __launch_bounds__(THREADS, 4) void evict_select_kernel(EvictArgs a) {
                 }
                 // the first list entry that moves is the first token that leaves; a lower bound at four tokens' grain
                 const uint64_t gaps = __builtin_amdgcn_ballot_w64(gap);
-                if (gaps != 0 && lane == 0) atomicMin(&sm_first, tile * kTile + 4 * (i * THREADS + 64 * wave + __builtin_ctzll(gaps)));
+                if (gaps != 0 && lane == 0) atomicMin(&sm_first, base + i * kGroup + 256 * wave + 4 * __builtin_ctzll(gaps));
             }
-            const uint32_t all = (uint32_t)__builtin_amdgcn_readlane((int)pair, 63);
+            const uint32_t all = sm_pre[groups * kWaves];
             sure += all & 0xffffu;
             ties += all >> 16;
+            __syncthreads();  // sm_cnt and sm_pre may be written again
         }
     }
-    // ---- weights in place: the tail; the row's counts
+    // ---- weights in place (otherwise they move with their tokens): list[r] >= r, so a tile of them overwrites nothing that
+    //      later ones read; then the tail, and the row's counts
     __syncthreads();
-    if (a.w && a.w == a.wo)
-        for (int64_t i = n + tid; i < min(a.wo_stride, (int64_t)a.max_seq_len); i += THREADS) a.wo[row * a.wo_stride + i] = 0.0f;
+    if (a.w && a.w == a.wo) {
+        float *wo = a.wo + row * a.wo_stride;
+        for (int r0 = 0; r0 < n; r0 += THREADS) {
+            const float x = r0 + tid < n ? w[list[r0 + tid]] : 0.0f;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (r0 + tid < n) wo[r0 + tid] = x;
+        }
+        __syncthreads();
+        for (int64_t i = n + tid; i < min(a.wo_stride, (int64_t)a.max_seq_len); i += THREADS) wo[i] = 0.0f;
+    }
     if (tid == 0) {
         a.info[2 * row] = n;
         a.info[2 * row + 1] = min(sm_first, n);
@@ -451,8 +481,8 @@ int hs_kv_evict(int fmt_fp8, const void *k_codes, const void *v_codes, const flo
     a.finish = std::max(std::min(budget, max_seq_len), kept ? budget : 0);
     if (weights_out) a.finish = std::max<int64_t>(a.finish, std::min<int64_t>(weights_out_stride, max_seq_len));
     hipStream_t st = (hipStream_t)stream;
-    if (max_seq_len <= 4 * kSelectNV * 256) evict_select_kernel<256><<<dim3(Hkv, B), 256, 0, st>>>(a);
-    else evict_select_kernel<1024><<<dim3(Hkv, B), 1024, 0, st>>>(a);
+    if (max_seq_len <= 8192) evict_select_kernel<8192><<<dim3(Hkv, B), 1024, 0, st>>>(a);
+    else evict_select_kernel<32768><<<dim3(Hkv, B), 1024, 0, st>>>(a);
     if (int rc = check_launch("kv_evict (selection)")) return rc;
     if (in_place) {
         const dim3 grid(2, Hkv, B);

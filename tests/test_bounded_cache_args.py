@@ -75,6 +75,10 @@ def test_attn_weights_refusals():
     assert _weights(ws=None) == hb.HS_ERR_WORKSPACE
     assert _weights(nbytes=16) == hb.HS_ERR_WORKSPACE
     assert _weights(ws=ctypes.c_void_p(0x100040)) == hb.HS_ERR_INVALID_ARGUMENT
+    lay = hb.contiguous_layout(2, 96, 128)
+    lay.k_block_table = lay.v_block_table = 0x5000000
+    lay.block_table_stride = 8
+    assert _weights(lay=lay) == hb.HS_ERR_INVALID_ARGUMENT                      # blocks of 96 tokens
     assert _weights(B=0) == hb.HS_OK and _weights(S=0, q=None, w=None) == hb.HS_OK
 
 
