@@ -287,7 +287,10 @@ __device__ __forceinline__ void finish_rows(const EvictArgs &a, int64_t row, int
     }
 }
 
-constexpr int kMoveTokens = 128;  // tokens of a workgroup
+// Tokens of a workgroup.  Few registers and many wavefronts beat more loads per thread: 64 x 8 rows of 1024 tokens (D = 128,
+// 290 MB moved) take 53-55 us with 64 tokens, 63-66 with 128, 131 with 256.  Loads may hit what the last attention left in
+// the caches (one stream of 32k tokens: 4.4 us, 6.1 with the streaming hint); stores stream past them.
+constexpr int kMoveTokens = 64;
 
 template <int D>
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
@@ -313,8 +316,8 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
         const bool k_ok = resolve(a.ka, b, t, ku, kslot), v_ok = resolve(a.va, b, t, vu, vslot);
         ok[p] = k_ok && v_ok;
         if (ok[p]) {
-            k[p] = __builtin_nontemporal_load((const u32x4 *)(a.kc + ku * a.ka.code_stride_seq + (int64_t)h * a.ka.code_stride_head + (int64_t)kslot * D + 16 * sub));
-            v[p] = __builtin_nontemporal_load((const u32x4 *)(a.vc + vu * a.va.code_stride_seq + (int64_t)h * a.va.code_stride_head + (int64_t)vslot * D + 16 * sub));
+            k[p] = *((const u32x4 *)(a.kc + ku * a.ka.code_stride_seq + (int64_t)h * a.ka.code_stride_head + (int64_t)kslot * D + 16 * sub));
+            v[p] = *((const u32x4 *)(a.vc + vu * a.va.code_stride_seq + (int64_t)h * a.va.code_stride_head + (int64_t)vslot * D + 16 * sub));
         }
     }
 #pragma unroll
@@ -328,7 +331,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
             __builtin_nontemporal_store(v[p], (u32x4 *)(a.vco + vu * a.vao.code_stride_seq + (int64_t)h * a.vao.code_stride_head + (int64_t)vslot * D + 16 * sub));
         }
     }
-    if (!a.fp8) {  // threads 0..127 the K scales of the tile, 128..255 the V scales
+    if (!a.fp8 && tid < 2 * kMoveTokens) {  // the K scales of the tile, then its V scales
         const int i = i0 + (tid & (kMoveTokens - 1)), which = tid / kMoveTokens;
         const KvAddr &src = which ? a.va : a.ka, &dst = which ? a.vao : a.kao;
         int64_t u;
