@@ -128,6 +128,18 @@ def lib():
         L.hs_attn_weights_workspace_bytes.argtypes = [ctypes.c_int32] * 6
         L.hs_kv_evict_workspace_bytes.restype = ctypes.c_size_t
         L.hs_kv_evict_workspace_bytes.argtypes = [ctypes.c_int32] * 4
+        p, i, z, ll, f = ctypes.c_void_p, ctypes.c_int32, ctypes.c_size_t, ctypes.c_int64, ctypes.c_float
+        # declared argument types take plain addresses and numbers: the calls below wrap nothing
+        for fn in (L.hs_decode_attn_int8, L.hs_decode_attn_fp8):
+            fn.argtypes = [p, p, p, p, p, p, p, p, p, z, i, i, i, i, i, f, p]
+        L.hs_decode_attn_phases.argtypes = [i, i] + L.hs_decode_attn_int8.argtypes
+        for fn in (L.hs_decode_step_int8, L.hs_decode_step_fp8):
+            fn.argtypes = [p, p, p, i, p, p, p, p, p, p, p, p, z, i, i, i, i, i, f, p]
+        for fn in (L.hs_prefill_attn_int8, L.hs_prefill_attn_fp8):
+            fn.argtypes = [p, p, p, p, p, p, p, p, i, p, i, i, i, i, i, f, i, p]
+        L.hs_decode_step_weights.argtypes = [i, p, p, p, i, p, p, p, p, p, p, p, p, p, ll, p, z, i, i, i, i, i, f, p]
+        L.hs_attn_weights.argtypes = [i, p, p, p, p, p, i, p, p, ll, p, z, i, i, i, i, i, i, f, p]
+        L.hs_kv_evict.argtypes = [i, p, p, p, p, p, p, p, ll, p, p, p, p, p, p, p, ll, p, i, i, i, p, z, i, i, i, i, p]
         _lib = L
     return _lib
 
@@ -156,9 +168,22 @@ def _ptr(t):
     return ctypes.c_void_p(t.data_ptr() if t is not None else None)
 
 
+_raw_stream = None
+
+
 def _stream():
-    import torch
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    """The current stream of the current device.  A serving loop's calls are as short as 10 us, so this takes torch's
+    handle itself instead of building a Stream object around it (2 us) where torch offers it."""
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        get, dev = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
+        _raw_stream = (lambda: get(dev())) if get and dev and torch.cuda.is_initialized() else (lambda: torch.cuda.current_stream().cuda_stream)
+    return ctypes.c_void_p(_raw_stream())
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
 
 
 def _dtype_code(t):
@@ -274,10 +299,10 @@ def decode_attn(q, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, 
         fn = lambda *a: fn0(int(fp8), int(phases), *a)
     else:
         fn = lib().hs_decode_attn_fp8 if fp8 else lib().hs_decode_attn_int8
-    check(fn(_ptr(q), _ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), ctypes.byref(layout),
-             _ptr(seq_lens), _ptr(out), _ptr(workspace),
-             ctypes.c_size_t(workspace.numel() * workspace.element_size() if workspace is not None else 0),
-             B, Hq, Hkv, D, ctypes.c_int32(max_seq_len), ctypes.c_float(softmax_scale), _stream()))
+    check(fn(q.data_ptr(), k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+             ctypes.addressof(layout), seq_lens.data_ptr(), out.data_ptr(), _addr(workspace),
+             workspace.numel() * workspace.element_size() if workspace is not None else 0, B, Hq, Hkv, D, max_seq_len,
+             softmax_scale, _stream()))
 
 
 def decode_attn_static(q, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, Hkv, max_seq_len, softmax_scale,
@@ -298,10 +323,10 @@ def decode_step(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, layout, s
     layout.decode_window, layout.attn_sinks = window, sinks
     assert k_new.shape == (B, 1, Hkv, D) and k_new.is_contiguous() and v_new.is_contiguous()
     fn = lib().hs_decode_step_fp8 if fp8 else lib().hs_decode_step_int8
-    check(fn(_ptr(q), _ptr(k_new), _ptr(v_new), _dtype_code(k_new), _ptr(k_codes), _ptr(v_codes), _ptr(k_scales),
-             _ptr(v_scales), ctypes.byref(layout), _ptr(seq_lens), _ptr(out), _ptr(workspace),
-             ctypes.c_size_t(workspace.numel() * workspace.element_size()), B, Hq, Hkv, D,
-             ctypes.c_int32(max_seq_len), ctypes.c_float(softmax_scale), _stream()))
+    check(fn(q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), _dtype_code(k_new), k_codes.data_ptr(), v_codes.data_ptr(),
+             k_scales.data_ptr(), v_scales.data_ptr(), ctypes.addressof(layout), seq_lens.data_ptr(), out.data_ptr(),
+             workspace.data_ptr(), workspace.numel() * workspace.element_size(), B, Hq, Hkv, D, max_seq_len, softmax_scale,
+             _stream()))
 
 
 def decode_step_rope(q, k_new, v_new, rope_sin, rope_cos, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out,
@@ -340,11 +365,11 @@ def decode_step_weights(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, l
     assert k_new is None or (k_new.shape == (B, 1, Hkv, D) and k_new.is_contiguous() and v_new.is_contiguous())
     stride = _weights_rows(weights_in, weights_out, B, Hkv)
     layout.decode_window, layout.attn_sinks = window, sinks
-    check(lib().hs_decode_step_weights(int(fp8), _ptr(q), _ptr(k_new), _ptr(v_new), HS_BF16 if k_new is None else _dtype_code(k_new),
-                                       _ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales), ctypes.byref(layout),
-                                       _ptr(seq_lens), _ptr(out), _ptr(weights_in), _ptr(weights_out), ctypes.c_int64(stride),
-                                       _ptr(workspace), ctypes.c_size_t(workspace.numel() * workspace.element_size()),
-                                       B, Hq, Hkv, D, ctypes.c_int32(max_seq_len), ctypes.c_float(softmax_scale), _stream()))
+    check(lib().hs_decode_step_weights(fp8, q.data_ptr(), _addr(k_new), _addr(v_new), HS_BF16 if k_new is None else _dtype_code(k_new),
+                                       k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                                       ctypes.addressof(layout), seq_lens.data_ptr(), out.data_ptr(), _addr(weights_in),
+                                       weights_out.data_ptr(), stride, workspace.data_ptr(),
+                                       workspace.numel() * workspace.element_size(), B, Hq, Hkv, D, max_seq_len, softmax_scale, _stream()))
 
 
 def attn_weights_workspace_bytes(B, S, Hq, Hkv, D, max_seq_len):
@@ -360,10 +385,9 @@ def attn_weights(q, k_codes, k_scales, layout, weights_in, weights_out, workspac
     assert positions is None or (str(positions.dtype) == "torch.int32" and positions.is_contiguous() and positions.numel() == B)
     stride = _weights_rows(weights_in, weights_out, B, Hkv)
     layout.prefill_window, layout.attn_sinks = window, sinks
-    check(lib().hs_attn_weights(int(fp8), _ptr(q), _ptr(k_codes), _ptr(k_scales), ctypes.byref(layout), _ptr(positions),
-                                ctypes.c_int32(start_pos), _ptr(weights_in), _ptr(weights_out), ctypes.c_int64(stride),
-                                _ptr(workspace), ctypes.c_size_t(workspace.numel() * workspace.element_size()),
-                                B, S, Hq, Hkv, D, ctypes.c_int32(max_seq_len), ctypes.c_float(softmax_scale), _stream()))
+    check(lib().hs_attn_weights(fp8, q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), ctypes.addressof(layout), _addr(positions),
+                                start_pos, _addr(weights_in), weights_out.data_ptr(), stride, workspace.data_ptr(),
+                                workspace.numel() * workspace.element_size(), B, S, Hq, Hkv, D, max_seq_len, softmax_scale, _stream()))
 
 
 def kv_evict_workspace_bytes(B, Hkv, budget, max_seq_len):
@@ -375,21 +399,20 @@ def kv_evict(cache, layout, seq_lens, weights, cache_out, layout_out, seq_lens_o
     """Keep `budget` tokens per (sequence, kv-head): the first `sinks`, the last `recent` and the heaviest of those between,
     moved to the front in their order.  cache, cache_out: (k_codes, v_codes, k_scales, v_scales); passing the same tensors
     and layout evicts in place.  weights, weights_out: fp32 [B, Hkv, stride] or None; kept: int32 [B, Hkv, budget] or None."""
-    B = seq_lens.numel()
-    codes = cache[0]
+    B, codes = seq_lens.numel(), cache[0]
     Hkv, D = codes.shape[1], codes.shape[3]
     for t in (weights, weights_out, kept, seq_lens, seq_lens_out):
         assert t is None or (t.is_contiguous() and t.element_size() == 4)
     assert kept is None or kept.shape == (B, Hkv, budget)
-    for t in (weights, weights_out):
-        assert t is None or t.shape[:2] == (B, Hkv)
-    check(lib().hs_kv_evict(int(fp8), *[_ptr(t) for t in cache], ctypes.byref(layout), _ptr(seq_lens), _ptr(weights),
-                            ctypes.c_int64(weights.shape[2] if weights is not None else 0), *[_ptr(t) for t in cache_out],
-                            ctypes.byref(layout_out), _ptr(seq_lens_out), _ptr(weights_out),
-                            ctypes.c_int64(weights_out.shape[2] if weights_out is not None else 0), _ptr(kept),
-                            ctypes.c_int32(budget), ctypes.c_int32(sinks), ctypes.c_int32(recent), _ptr(workspace),
-                            ctypes.c_size_t(workspace.numel() * workspace.element_size()), B, Hkv, D,
-                            ctypes.c_int32(max_seq_len), _stream()))
+    assert weights is None or weights.shape[:2] == (B, Hkv)
+    assert weights_out is None or weights_out.shape[:2] == (B, Hkv)
+    kc, vc, ks, vs = cache
+    kco, vco, kso, vso = cache_out
+    check(lib().hs_kv_evict(fp8, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), ctypes.addressof(layout),
+                            seq_lens.data_ptr(), _addr(weights), weights.shape[2] if weights is not None else 0, kco.data_ptr(),
+                            vco.data_ptr(), kso.data_ptr(), vso.data_ptr(), ctypes.addressof(layout_out), seq_lens_out.data_ptr(),
+                            _addr(weights_out), weights_out.shape[2] if weights_out is not None else 0, _addr(kept), budget, sinks,
+                            recent, workspace.data_ptr(), workspace.numel() * workspace.element_size(), B, Hkv, D, max_seq_len, _stream()))
 
 
 def prefill_split_workspace(B, S, Hq, Hkv, D, device="cuda:0"):
@@ -457,10 +480,8 @@ def prefill_attn(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, layout, 
                  ctypes.c_float(softmax_scale), int(bool(quantize_on_write)), _stream()))
         return
     fn = lib().hs_prefill_attn_fp8 if fp8 else lib().hs_prefill_attn_int8
-    check(fn(_ptr(q), _ptr(k_new), _ptr(v_new), _ptr(k_codes), _ptr(v_codes), _ptr(k_scales),
-                                     _ptr(v_scales), ctypes.byref(layout), ctypes.c_int32(hist_len), _ptr(out),
-                                     B, S, Hq, Hkv, D, ctypes.c_float(softmax_scale), int(bool(quantize_on_write)),
-                                     _stream()))
+    check(fn(q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), _addr(k_codes), _addr(v_codes), _addr(k_scales), _addr(v_scales),
+             ctypes.addressof(layout), hist_len, out.data_ptr(), B, S, Hq, Hkv, D, softmax_scale, bool(quantize_on_write), _stream()))
 
 
 def deltanet_forward(q, k, v, g, beta, state, out, q_scale, l2norm=False):
