@@ -481,6 +481,25 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
                 }
     };
 
+    // kMode 2: the scores wait in this wavefront's part of the merge buffer (free until the walk is over) and go to memory
+    // `hold` steps at a time, whole lines, streamed past the caches.  A store in the stream of K/V loads makes later loads
+    // wait for it: written with every step the scores cost 63 us of 244 at 64 x 8192 tokens (67 MB), held back 45, and
+    // streamed as well 25.
+    float *const held_scores = &sm_o[wave][0][0];
+    const int hold = 16 * (CW + 4) / (G * kStep);
+    int held = 0;
+    auto write_scores = [&](int last_step) {  // held steps end at last_step, kWavesPerWg apart
+        __builtin_amdgcn_wave_barrier();
+        constexpr int kPieces = kStep / 4;
+        for (int i = lane; i < held * G * kPieces; i += 64) {
+            const int piece = i % kPieces, g = (i / kPieces) % G, s = i / (kPieces * G);
+            const int t = t_begin + (last_step - (held - 1 - s) * kWavesPerWg) * kStep + 4 * piece;
+            __builtin_nontemporal_store(*(const float4v *)(held_scores + 4 * i), (float4v *)(a.logits + ((int64_t)b * a.Hq + h * G + g) * a.logit_stride + t));
+        }
+        __builtin_amdgcn_wave_barrier();
+        held = 0;
+    };
+
     auto compute_stage = [&](const Stage<kD> &st, int step) {
         const int t0 = actual(t_begin + step * kStep);
         // ---- token scales: lane (li, lq) needs those of tokens 16u + 4*lq + r, the rows of its score registers.
@@ -559,10 +578,11 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
         }
         if constexpr (kMode == 2) {
             if (li < G) {
-                float *row = a.logits + ((int64_t)b * a.Hq + h * G + li) * a.logit_stride + t_begin + step * kStep + 4 * lq;
+                float *row = held_scores + (held * G + li) * kStep + 4 * lq;
 #pragma unroll
                 for (int u = 0; u < NT; ++u) *(float4v *)(row + 16 * u) = (float4v){sc[4 * u], sc[4 * u + 1], sc[4 * u + 2], sc[4 * u + 3]};
             }
+            if (++held == hold) write_scores(step);
         }
         // ---- online softmax (max shared by the 4 lanes of a head)
         float mx = sc[0];
@@ -697,6 +717,9 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
         compute_stage(sb, n1);
         step = n2;
     }
+
+    if constexpr (kMode == 2)
+        if (held > 0) write_scores(wave + (nsteps - 1 - wave) / kWavesPerWg * kWavesPerWg);
 
     // ---- the next item's first tiles travel while this one is merged and written out
     if (kPreloadNext && has_next) {
@@ -854,11 +877,11 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
 // 256 threads: D/4 column lanes (four output elements each) x 1024/D chunk lanes, so the partials of a long
 // sequence (up to 128 chunks) are read by many lanes at once instead of one after the other; the chunk lanes meet
 // in LDS.  D is 64, 128 or 256.
-__global__ __launch_bounds__(256) void decode_merge_kernel(const float *part_o, const float *part_ml,
+__device__ __forceinline__ void merge_row(int hq, int b, const float *part_o, const float *part_ml,
                                                           const int32_t *seq_lens, uint16_t *out, const uint16_t *out_gate, int Hq, int nchunks,
                                                           int chunk_tokens, int max_seq_len, int kD, int B, int pieces,
                                                           int min_granules, int window, int sinks) {
-    const int hq = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    const int tid = threadIdx.x;
     const int L = visible_line(min(seq_lens[b], max_seq_len), window, sinks, 4096 / kD).len;
     __shared__ float sm_max[4], sm_l[16];
     __shared__ __attribute__((aligned(16))) float sm_o[1024];
@@ -924,15 +947,31 @@ __global__ __launch_bounds__(256) void decode_merge_kernel(const float *part_o, 
     }
 }
 
+__global__ __launch_bounds__(256) void decode_merge_kernel(const float *part_o, const float *part_ml,
+                                                          const int32_t *seq_lens, uint16_t *out, const uint16_t *out_gate, int Hq, int nchunks,
+                                                          int chunk_tokens, int max_seq_len, int kD, int B, int pieces,
+                                                          int min_granules, int window, int sinks) {
+    merge_row(blockIdx.x, blockIdx.y, part_o, part_ml, seq_lens, out, out_gate, Hq, nchunks, chunk_tokens, max_seq_len, kD, B,
+              pieces, min_granules, window, sinks);
+}
+
 // The softmax weights of one decode step added up over the query heads of each kv-head (kMode 2 above):
 //   out[b, h, t] = in[b, h, t] + sum_g exp2(logit[b, hG + g, t] - m_g) / l_g,   t < L
 // with m_g and l_g joined from the chunk partials.  Grid (token blocks of 1024, kv-heads, sequences), four tokens per
-// thread.  Tokens outside the window keep their value.
-__global__ __launch_bounds__(256) void decode_weights_kernel(const float *logits, int64_t logit_stride, const float *part_ml,
-                                                            const int32_t *seq_lens, const float *in, float *out,
-                                                            int64_t stride, int Hq, int G, int nchunks, int chunk_tokens,
-                                                            int max_seq_len, int window, int sinks, int step) {
-    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63;
+// thread.  Tokens outside the window keep their value.  Where the sequences are split (part_o), G more blocks of every
+// (kv-head, sequence) merge the heads' chunk partials into the output: one launch instead of two.
+__global__ __launch_bounds__(256) void decode_weights_kernel(const float *logits, int64_t logit_stride, const float *part_o,
+                                                            const float *part_ml, const int32_t *seq_lens, const float *in,
+                                                            float *out, int64_t stride, uint16_t *attn_out,
+                                                            const uint16_t *out_gate, int Hq, int G, int kD, int nchunks,
+                                                            int chunk_tokens, int max_seq_len, int window, int sinks) {
+    const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, lane = tid & 63, step = 4096 / kD;
+    const int blocks = (max_seq_len + 1023) / 1024;
+    if ((int)blockIdx.x >= blocks) {
+        merge_row(h * G + blockIdx.x - blocks, b, part_o, part_ml, seq_lens, attn_out, out_gate, Hq, nchunks, chunk_tokens,
+                  max_seq_len, kD, gridDim.z, 0, 0, window, sinks);
+        return;
+    }
     const int L = min(seq_lens[b], max_seq_len);
     const int t0 = blockIdx.x * 1024;
     if (t0 >= L) return;
@@ -1211,17 +1250,17 @@ static int launch_decode(bool fp8, int phases, const NewToken &nt, const void *q
 #undef HS_DECODE_LAUNCH
         if (int rc = check_launch("decode_attn")) return rc;
     }
+    if (weights) {
+        decode_weights_kernel<<<dim3((max_seq_len + 1023) / 1024 + (a.direct ? 0 : a.G), Hkv, B), 256, 0, stream>>>(
+            a.logits, a.logit_stride, a.part_o, a.part_ml, seq_lens, wt.in, wt.out, wt.stride, a.out, a.out_gate, Hq, a.G, D,
+            a.nchunks, a.chunk_tokens, max_seq_len, a.window, a.sinks);
+        return check_launch("decode_weights");
+    }
     if ((phases & 2) && !a.direct) {
         decode_merge_kernel<<<dim3(Hq, B), 256, 0, stream>>>(a.part_o, a.part_ml, seq_lens, (uint16_t *)out, a.out_gate, Hq,
                                                                a.nchunks, a.chunk_tokens, max_seq_len, D, B,
                                                                a.balanced ? a.pieces : 0, a.min_granules, a.window, a.sinks);
-        if (int rc = check_launch("decode_merge")) return rc;
-    }
-    if (weights) {
-        decode_weights_kernel<<<dim3((max_seq_len + 1023) / 1024, Hkv, B), 256, 0, stream>>>(
-            a.logits, a.logit_stride, a.part_ml, seq_lens, wt.in, wt.out, wt.stride, Hq, a.G, a.nchunks, a.chunk_tokens,
-            max_seq_len, a.window, a.sinks, step);
-        return check_launch("decode_weights");
+        return check_launch("decode_merge");
     }
     return HS_OK;
 }

@@ -379,7 +379,7 @@ HS_API int hs_decode_attn_phases(int fmt_fp8, int phases, const void *q, const v
 /* hs_decode_step_* (k_new, v_new: one new token per sequence, written at seq_lens[b] - 1 first; both NULL:
  * hs_decode_attn_*) together with the weights of its Hq queries.  fmt_fp8 as in hs_decode_attn_phases; decode_window,
  * attn_sinks and out_gate of the layout apply (a token the window hides receives nothing).  q and k_new arrive
- * normalised and rotated.  Three launches at most; the workspace is hs_decode_weights_workspace_bytes(...) bytes,
+ * normalised and rotated.  Two launches; the workspace is hs_decode_weights_workspace_bytes(...) bytes,
  * 256-byte aligned (the scores pass through it: 4 bytes per query head and token). */
 HS_API size_t hs_decode_weights_workspace_bytes(int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_seq_len);
 HS_API int hs_decode_step_weights(int fmt_fp8, const void *q, const void *k_new, const void *v_new, int src_dtype,
