@@ -40,6 +40,64 @@ __device__ __forceinline__ uint32_t weight_key(float f) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
+// What goes with the codes of list entries [i0, i1): the caller's list, the weights and the zeros behind them (weights in
+// place have been moved by the selection).  `threads` threads take part.
+__device__ __forceinline__ void finish_rows(const EvictArgs &a, int64_t row, int n, int i0, int i1, int tid, int threads) {
+    const int32_t *list = a.list + row * a.budget;
+    const bool move_weights = a.wo != nullptr && a.w != a.wo;
+    if (!move_weights && a.kept == nullptr) return;
+    const int64_t w_end = min(a.wo_stride, (int64_t)a.max_seq_len);
+    for (int i = i0 + tid; i < i1; i += threads) {
+        const int t = i < n ? list[i] : -1;
+        if (a.kept && i < a.budget) a.kept[row * a.budget + i] = t;
+        if (move_weights && i < w_end) a.wo[row * a.wo_stride + i] = t >= 0 && a.w ? a.w[row * a.w_stride + t] : 0.0f;
+    }
+}
+
+// Codes and scales of list entries [i0, i0 + TOKENS) of a row, by THREADS threads.
+template <int D, int THREADS, int TOKENS>
+__device__ __forceinline__ void move_tile(const EvictArgs &a, int64_t row, int b, int h, int n, int i0, int tid) {
+    constexpr int LPR = D / 16, RPP = THREADS / LPR, PASSES = TOKENS / RPP;  // lanes per row, rows per pass
+    const int32_t *list = a.list + row * a.budget;
+    const int sub = tid % LPR, r = tid / LPR;
+    u32x4 k[PASSES], v[PASSES];
+    bool ok[PASSES];
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+        const int i = i0 + p * RPP + r;
+        int64_t ku, vu;
+        int kslot, vslot;
+        const int t = i < n ? list[i] : -1;
+        const bool k_ok = resolve(a.ka, b, t, ku, kslot), v_ok = resolve(a.va, b, t, vu, vslot);
+        ok[p] = k_ok && v_ok;
+        if (ok[p]) {
+            k[p] = *((const u32x4 *)(a.kc + ku * a.ka.code_stride_seq + (int64_t)h * a.ka.code_stride_head + (int64_t)kslot * D + 16 * sub));
+            v[p] = *((const u32x4 *)(a.vc + vu * a.va.code_stride_seq + (int64_t)h * a.va.code_stride_head + (int64_t)vslot * D + 16 * sub));
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < PASSES; ++p) {
+        const int i = i0 + p * RPP + r;
+        int64_t ku, vu;
+        int kslot, vslot;
+        const bool k_ok = resolve(a.kao, b, i, ku, kslot), v_ok = resolve(a.vao, b, i, vu, vslot);
+        if (ok[p] && k_ok && v_ok) {
+            __builtin_nontemporal_store(k[p], (u32x4 *)(a.kco + ku * a.kao.code_stride_seq + (int64_t)h * a.kao.code_stride_head + (int64_t)kslot * D + 16 * sub));
+            __builtin_nontemporal_store(v[p], (u32x4 *)(a.vco + vu * a.vao.code_stride_seq + (int64_t)h * a.vao.code_stride_head + (int64_t)vslot * D + 16 * sub));
+        }
+    }
+    if (!a.fp8 && tid < 2 * TOKENS) {  // the K scales of the tile, then its V scales
+        const int i = i0 + (tid & (TOKENS - 1)), which = tid / TOKENS;
+        const KvAddr &src = which ? a.va : a.ka, &dst = which ? a.vao : a.kao;
+        int64_t u;
+        int slot;
+        if (i < n && resolve(src, b, list[i], u, slot)) {
+            const float s = (which ? a.vs : a.ks)[u * src.scale_stride_seq + (int64_t)h * src.scale_stride_head + slot];
+            if (resolve(dst, b, i, u, slot)) (which ? a.vso : a.kso)[u * dst.scale_stride_seq + (int64_t)h * dst.scale_stride_head + slot] = s;
+        }
+    }
+}
+
 // Inclusive sum over the wavefront's lanes on the vector pipe (row shifts inside sixteen lanes, then the broadcasts of
 // lane 15 and of lane 31): six dependent additions instead of six trips through the LDS crossbar.
 __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
@@ -58,9 +116,10 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 // tile at a time.  A row is a chain of short steps -- three histograms with a scan each, one scan for the list -- so what
 // it costs is latency: the scans run on the vector pipe, a pass counts without branches (what it
 // does not count goes to a place of the lane's own), and sixteen wavefronts hide each other's latencies (with four per
-// row and 32 weights a thread: 25 us at 64 x 8 rows of 8192 tokens against @).
+// row and 32 weights a thread: 25 us at 64 x 8 rows of 8192 tokens, 14 now).
 constexpr uint32_t kProtected = 0xffffffffu, kZeroKey = 0x80000000u;
-template <int TILE>
+// MOVE: head_dim of the codes if the workgroup goes on to move its row's tokens itself, 0 if evict_move_kernel does.
+template <int TILE, int MOVE>
 __global__ __launch_bounds__(1024) void evict_select_kernel(EvictArgs a) {
     constexpr int THREADS = 1024;
     constexpr uint32_t kCand = 1024;
@@ -267,23 +326,16 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvictArgs a) {
         __syncthreads();
         for (int64_t i = n + tid; i < min(a.wo_stride, (int64_t)a.max_seq_len); i += THREADS) wo[i] = 0.0f;
     }
-    if (tid == 0) {
+    if constexpr (MOVE != 0) {
+        __syncthreads();  // the list
+        constexpr int kTokens = 2 * (THREADS / (MOVE / 16));
+        if (h == 0 && tid == 0) a.seq_lens_out[b] = n;  // (the lengths the other heads read are another array)
+        if (a.fp8 && tid < 2) (tid ? a.vso : a.kso)[row] = (tid ? a.vs : a.ks)[row];
+        finish_rows(a, row, n, 0, a.finish, tid, THREADS);
+        for (int i0 = 0; i0 < n; i0 += kTokens) move_tile<MOVE, THREADS, kTokens>(a, row, b, h, n, i0, tid);
+    } else if (tid == 0) {
         a.info[2 * row] = n;
         a.info[2 * row + 1] = min(sm_first, n);
-    }
-}
-
-// What goes with the codes of list entries [i0, i1): the caller's list, the weights and the zeros behind them (weights in
-// place have been moved by the selection).  `threads` threads take part.
-__device__ __forceinline__ void finish_rows(const EvictArgs &a, int64_t row, int n, int i0, int i1, int tid, int threads) {
-    const int32_t *list = a.list + row * a.budget;
-    const bool move_weights = a.wo != nullptr && a.w != a.wo;
-    if (!move_weights && a.kept == nullptr) return;
-    const int64_t w_end = min(a.wo_stride, (int64_t)a.max_seq_len);
-    for (int i = i0 + tid; i < i1; i += threads) {
-        const int t = i < n ? list[i] : -1;
-        if (a.kept && i < a.budget) a.kept[row * a.budget + i] = t;
-        if (move_weights && i < w_end) a.wo[row * a.wo_stride + i] = t >= 0 && a.w ? a.w[row * a.w_stride + t] : 0.0f;
     }
 }
 
@@ -294,53 +346,13 @@ constexpr int kMoveTokens = 64;
 
 template <int D>
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
-    constexpr int LPR = D / 16, RPP = 256 / LPR, PASSES = kMoveTokens / RPP;  // lanes per row, rows per pass
     const int h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
     const int64_t row = (int64_t)b * a.Hkv + h;
-    const int n = a.info[2 * row];
+    const int n = a.info[2 * row], i0 = blockIdx.x * kMoveTokens;
     if (blockIdx.x == 0 && h == 0 && tid == 0) a.seq_lens_out[b] = n;
     if (blockIdx.x == 0 && a.fp8 && tid < 2) (tid ? a.vso : a.kso)[row] = (tid ? a.vs : a.ks)[row];
-    const int i0 = blockIdx.x * kMoveTokens;
     finish_rows(a, row, n, i0, i0 + kMoveTokens, tid, 256);
-    if (i0 >= n) return;
-    const int32_t *list = a.list + row * a.budget;
-    const int sub = tid % LPR, r = tid / LPR;
-    u32x4 k[PASSES], v[PASSES];
-    bool ok[PASSES];
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-        const int i = i0 + p * RPP + r;
-        int64_t ku, vu;
-        int kslot, vslot;
-        const int t = i < n ? list[i] : -1;
-        const bool k_ok = resolve(a.ka, b, t, ku, kslot), v_ok = resolve(a.va, b, t, vu, vslot);
-        ok[p] = k_ok && v_ok;
-        if (ok[p]) {
-            k[p] = *((const u32x4 *)(a.kc + ku * a.ka.code_stride_seq + (int64_t)h * a.ka.code_stride_head + (int64_t)kslot * D + 16 * sub));
-            v[p] = *((const u32x4 *)(a.vc + vu * a.va.code_stride_seq + (int64_t)h * a.va.code_stride_head + (int64_t)vslot * D + 16 * sub));
-        }
-    }
-#pragma unroll
-    for (int p = 0; p < PASSES; ++p) {
-        const int i = i0 + p * RPP + r;
-        int64_t ku, vu;
-        int kslot, vslot;
-        const bool k_ok = resolve(a.kao, b, i, ku, kslot), v_ok = resolve(a.vao, b, i, vu, vslot);
-        if (ok[p] && k_ok && v_ok) {
-            __builtin_nontemporal_store(k[p], (u32x4 *)(a.kco + ku * a.kao.code_stride_seq + (int64_t)h * a.kao.code_stride_head + (int64_t)kslot * D + 16 * sub));
-            __builtin_nontemporal_store(v[p], (u32x4 *)(a.vco + vu * a.vao.code_stride_seq + (int64_t)h * a.vao.code_stride_head + (int64_t)vslot * D + 16 * sub));
-        }
-    }
-    if (!a.fp8 && tid < 2 * kMoveTokens) {  // the K scales of the tile, then its V scales
-        const int i = i0 + (tid & (kMoveTokens - 1)), which = tid / kMoveTokens;
-        const KvAddr &src = which ? a.va : a.ka, &dst = which ? a.vao : a.kao;
-        int64_t u;
-        int slot;
-        if (i < n && resolve(src, b, list[i], u, slot)) {
-            const float s = (which ? a.vs : a.ks)[u * src.scale_stride_seq + (int64_t)h * src.scale_stride_head + slot];
-            if (resolve(dst, b, i, u, slot)) (which ? a.vso : a.kso)[u * dst.scale_stride_seq + (int64_t)h * dst.scale_stride_head + slot] = s;
-        }
-    }
+    if (i0 < n) move_tile<D, 256, kMoveTokens>(a, row, b, h, n, i0, tid);
 }
 
 // In place: list[i] >= i, so a tile of destinations can only overlap sources of its own tile and of earlier ones.  Every
@@ -484,9 +496,23 @@ int hs_kv_evict(int fmt_fp8, const void *k_codes, const void *v_codes, const flo
     a.finish = std::max(std::min(budget, max_seq_len), kept ? budget : 0);
     if (weights_out) a.finish = std::max<int64_t>(a.finish, std::min<int64_t>(weights_out_stride, max_seq_len));
     hipStream_t st = (hipStream_t)stream;
-    if (max_seq_len <= 8192) evict_select_kernel<8192><<<dim3(Hkv, B), 1024, 0, st>>>(a);
-    else evict_select_kernel<32768><<<dim3(Hkv, B), 1024, 0, st>>>(a);
+    // One launch where there is little to move: a workgroup per row then moves its tokens itself.  (5 x 4 rows of 512 tokens
+    // of 64 codes: a call every 11.3 us, 15.7 in two launches, whose second one costs the host as much as the GPU; 64 x 8
+    // rows of 1024 tokens of 128: 73.6 us of kernel against 68.9; 8 rows of 4096 tokens: 51 against 34.)
+    const int64_t row_bytes = (int64_t)a.finish * D;
+    const bool one = !in_place && seq_lens_out != seq_lens && row_bytes <= 65536 && (int64_t)B * Hkv * row_bytes <= (8 << 20);
+#define HS_EVICT_SELECT(M)                                                                          \
+    do {                                                                                            \
+        if (max_seq_len <= 8192) evict_select_kernel<8192, M><<<dim3(Hkv, B), 1024, 0, st>>>(a);    \
+        else evict_select_kernel<32768, M><<<dim3(Hkv, B), 1024, 0, st>>>(a);                       \
+    } while (0)
+    if (!one) HS_EVICT_SELECT(0);
+    else if (D == 64) HS_EVICT_SELECT(64);
+    else if (D == 128) HS_EVICT_SELECT(128);
+    else HS_EVICT_SELECT(256);
+#undef HS_EVICT_SELECT
     if (int rc = check_launch("kv_evict (selection)")) return rc;
+    if (one) return HS_OK;
     if (in_place) {
         const dim3 grid(2, Hkv, B);
         if (D == 64) evict_inplace_kernel<64><<<grid, 1024, 0, st>>>(a);
