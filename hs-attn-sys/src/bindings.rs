@@ -172,6 +172,10 @@ extern "C" {
     pub fn hs_cache_decode_attention(c: *mut hs_cache, q: *const c_void, out: *mut c_void, num_q_heads: i32, softmax_scale: f32, stream: hs_stream_t) -> c_int;
     pub fn hs_cache_decode_step(c: *mut hs_cache, q: *const c_void, k_new: *const c_void, v_new: *const c_void, dtype: c_int, out: *mut c_void, num_q_heads: i32, softmax_scale: f32, stream: hs_stream_t) -> c_int;
     pub fn hs_cache_prefill(c: *mut hs_cache, q: *const c_void, new_keys: *const c_void, new_values: *const c_void, out: *mut c_void, batch: i32, seq_len: i32, num_q_heads: i32, num_kv_heads: i32, head_dim: i32, start_pos: i64, softmax_scale: f32, stream: hs_stream_t) -> c_int;
+    pub fn hs_cache_set_window(c: *mut hs_cache, window: i32, sinks: i32) -> c_int;
+    pub fn hs_cache_track_weights(c: *mut hs_cache, on: c_int) -> c_int;
+    pub fn hs_cache_get_weights(c: *mut hs_cache, weights_out: *mut f32, stream: hs_stream_t) -> c_int;
+    pub fn hs_cache_evict(c: *mut hs_cache, budget: i32, sinks: i32, recent: i32, stream: hs_stream_t) -> c_int;
     pub fn hs_cache_enable_prompt_scratch(c: *mut hs_cache, max_prompt_tokens: i64);
     pub fn hs_cache_drop_prompt_scratch(c: *mut hs_cache);
     pub fn hs_cache_prompt_copy_active(c: *const hs_cache) -> c_int;

@@ -23,10 +23,6 @@ namespace hs {
 
 constexpr float kWLog2e = 1.4426950408889634f;
 constexpr int kWStep = 64;       // keys of a step of the first kernel
-#ifndef CHN
-#define CHN 1024
-#define CHM 512
-#endif
 constexpr int kCStepMax = 128;   // columns of a step of the second (64 at head_dim 256)
 constexpr int kWThreads = 256;   // both kernels
 
@@ -619,15 +615,15 @@ static WeightsPlan plan_weights(int B, int S, int Hq, int Hkv, int D, int max_se
     p.col_blocks = (p.cols + wg_cols - 1) / wg_cols;
     p.key_blocks = ((int64_t)max_seq_len + wg_keys - 1) / wg_keys;
     // First kernel: few columns (an observation window) leave most CUs idle unless the keys are split, into chunks of
-    // at least 512.
-    const int64_t want = std::max<int64_t>(1, CHN / std::max<int64_t>(1, units * p.col_blocks));
+    // at least 512 (8 units, 128 columns, 32768 keys, us: 21.8 with chunks of 512, 23.4 with 256, 28.7 with 128).
+    const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(1, units * p.col_blocks));
     int64_t ct = ((int64_t)max_seq_len + want - 1) / want;
-    ct = std::max<int64_t>(CHM, (ct + kWStep - 1) / kWStep * kWStep);
+    ct = std::max<int64_t>(512, (ct + kWStep - 1) / kWStep * kWStep);
     p.chunk_tokens = (int)std::min<int64_t>(ct, ((int64_t)max_seq_len + kWStep - 1) / kWStep * kWStep);
     p.key_chunks = (int)(((int64_t)max_seq_len + p.chunk_tokens - 1) / p.chunk_tokens);
     // Second kernel: two workgroups are resident on each of 256 CUs, and each of them should come round twice: started in
     // order of their work, long items then meet short ones and the causal triangle evens out (4 x 4096 tokens, 16 key
-    // blocks on 32 units, us: @1 one share of the columns, @2 two, @4 four).
+    // blocks on 32 units, us: 369 with one share of the columns, 305 with two, 308 with four).
     const int64_t items = units * p.key_blocks, steps = (p.cols + kCStepMax - 1) / kCStepMax;
     p.segments = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(steps, 16), (1024 + items - 1) / items));
     p.part_stride = p.key_blocks * wg_keys;

@@ -19,6 +19,18 @@ inline hipError_t fill_i32(int32_t *p, int32_t n, int32_t v, hipStream_t stream)
     return hipGetLastError();
 }
 
+// Columns [from, to) of `rows` rows of `stride` floats.
+static __global__ void zero_columns_kernel(float *p, int64_t rows, int64_t stride, int64_t from, int64_t to) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, n = to - from;
+    if (i < rows * n) p[i / n * stride + from + i % n] = 0.0f;
+}
+
+inline hipError_t zero_columns(float *p, int64_t rows, int64_t stride, int64_t from, int64_t to, hipStream_t stream) {
+    if (rows <= 0 || to <= from) return hipSuccess;
+    zero_columns_kernel<<<(unsigned)((rows * (to - from) + 255) / 256), 256, 0, stream>>>(p, rows, stride, from, to);
+    return hipGetLastError();
+}
+
 // fp8 paged batch: the rows of a batch keep their per-kv-head scales in buffers of their own ([2][Hkv], K then V);
 // the decode entry point wants them as [n][Hkv] arrays.
 static __global__ void gather_head_scales_kernel(const float *const *rows, float *k_out, float *v_out, int32_t n, int32_t hkv) {

@@ -36,8 +36,12 @@ void LayerKVCache::drop_prompt_scratch() {
 
 void LayerKVCache::release() {
     drop_prompt_scratch();
-    for (void *p : {k_codes_, v_codes_, (void *)k_scales_, (void *)v_scales_, (void *)seq_lens_dev_, workspace_})
+    for (void *p : {k_codes_, v_codes_, (void *)k_scales_, (void *)v_scales_, (void *)seq_lens_dev_, workspace_, (void *)weights_, bound_ws_})
         if (p) (void)hipFree(p);
+    weights_ = nullptr;
+    bound_ws_ = nullptr;
+    weights_stride_ = 0;
+    weights_dirty_ = bound_ws_bytes_ = 0;
     k_codes_ = v_codes_ = workspace_ = nullptr;
     k_scales_ = v_scales_ = nullptr;
     seq_lens_dev_ = nullptr;
@@ -64,6 +68,8 @@ Status LayerKVCache::ensure_storage(int32_t batch, int32_t heads, int32_t dim) {
     layout_.scale_stride_head = (int64_t)cap_s;
     layout_.scale_stride_seq = (int64_t)cap_s * heads;
     layout_.capacity_tokens = (int32_t)cap;
+    layout_.decode_window = window_;
+    layout_.attn_sinks = sinks_;
     const size_t code_bytes = (size_t)batch * heads * cap * dim;
     const size_t scale_bytes = quant_type_ == KVQuantType::Fp8 ? (size_t)batch * heads * 4 : (size_t)batch * heads * cap_s * 4;
     hipError_t e;
@@ -98,6 +104,90 @@ Status LayerKVCache::ensure_scratch(int32_t hq, int32_t batch, hs_stream_t strea
     return hip_err(fill_i32(seq_lens_dev_, batch, (int32_t)seq_pos, (hipStream_t)stream), "setting the sequence lengths");
 }
 
+Status LayerKVCache::set_window(int32_t window, int32_t sinks) {
+    if (window < 0 || sinks < 0) return err(HS_ERR_INVALID_ARGUMENT, "negative window or sinks");
+    layout_.decode_window = window_ = window;
+    layout_.attn_sinks = sinks_ = sinks;
+    return {};
+}
+
+Status LayerKVCache::track_weights(bool on) {
+    track_ = on;
+    if (!on && weights_) {
+        // a step on some stream may still add to them
+        if (hipError_t e = hipDeviceSynchronize(); e != hipSuccess) return hip_err(e, "waiting before the weights are freed");
+        (void)hipFree(weights_);
+        weights_ = nullptr;
+        weights_stride_ = 0;
+        weights_dirty_ = 0;
+    }
+    return {};
+}
+
+// The rows (when tracking) and a workspace of at least `bytes`, which only ever grows.
+Status LayerKVCache::ensure_weights(size_t bytes, hs_stream_t stream) {
+    if (track_ && !weights_) {
+        weights_stride_ = (int64_t)((max_seq_len + 3) / 4 * 4);
+        const size_t n = (size_t)batch_ * heads_ * weights_stride_;
+        if (hipError_t e = hipMalloc((void **)&weights_, n * sizeof(float)); e != hipSuccess) {
+            weights_ = nullptr;
+            weights_stride_ = 0;
+            return hip_err(e, "allocating the weights");
+        }
+        if (hipError_t e = zero_columns(weights_, (int64_t)batch_ * heads_, weights_stride_, 0, weights_stride_, (hipStream_t)stream); e != hipSuccess)
+            return hip_err(e, "clearing the weights");
+        weights_dirty_ = 0;
+    }
+    if (bytes > bound_ws_bytes_) {
+        if (bound_ws_) {
+            if (hipError_t e = hipDeviceSynchronize(); e != hipSuccess) return hip_err(e, "waiting before the workspace grows");
+            (void)hipFree(bound_ws_);
+        }
+        bound_ws_ = nullptr;
+        bound_ws_bytes_ = 0;
+        if (hipError_t e = hipMalloc(&bound_ws_, bytes); e != hipSuccess) {
+            bound_ws_ = nullptr;
+            return hip_err(e, "allocating the workspace");
+        }
+        bound_ws_bytes_ = bytes;
+    }
+    return {};
+}
+
+// Tokens from `from` on are about to be cached anew: they start without weight.
+Status LayerKVCache::clean_weights(size_t from, hs_stream_t stream) {
+    if (!weights_ || weights_dirty_ <= from) return {};
+    const size_t to = weights_dirty_;
+    weights_dirty_ = from;
+    return hip_err(zero_columns(weights_, (int64_t)batch_ * heads_, weights_stride_, (int64_t)from, (int64_t)to, (hipStream_t)stream), "clearing the weights");
+}
+
+Status LayerKVCache::get_weights(float *out, hs_stream_t stream) const {
+    if (!k_codes_ || seq_pos == 0) return err(HS_ERR_INVALID_ARGUMENT, "Cache is empty");
+    if (!weights_) return err(HS_ERR_INVALID_ARGUMENT, "no weights have been counted: track_weights() comes before the calls that add them");
+    if (!out) return err(HS_ERR_INVALID_ARGUMENT, "null buffer");
+    return hip_err(hipMemcpy2DAsync(out, seq_pos * sizeof(float), weights_, weights_stride_ * sizeof(float), seq_pos * sizeof(float),
+                                    (size_t)batch_ * heads_, hipMemcpyDeviceToDevice, (hipStream_t)stream), "copying the weights");
+}
+
+Status LayerKVCache::evict(int32_t budget, int32_t sinks, int32_t recent, hs_stream_t stream) {
+    if (!k_codes_ || seq_pos == 0) return err(HS_ERR_INVALID_ARGUMENT, "Cache is empty");
+    if (budget <= 0 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
+        return err(HS_ERR_INVALID_ARGUMENT, "need budget > 0 and 0 <= sinks + recent <= budget");
+    if ((size_t)budget >= seq_pos) return {};
+    if (Status s = ensure_weights(hs_kv_evict_workspace_bytes(batch_, heads_, budget, (int32_t)seq_pos), stream); !s.ok()) return s;
+    if (hipError_t e = fill_i32(seq_lens_dev_, batch_, (int32_t)seq_pos, (hipStream_t)stream); e != hipSuccess)
+        return hip_err(e, "setting the sequence lengths");
+    const int rc = hs_kv_evict(quant_type_ == KVQuantType::Fp8, k_codes_, v_codes_, k_scales_, v_scales_, &layout_, seq_lens_dev_, weights_,
+                               weights_stride_, k_codes_, v_codes_, k_scales_, v_scales_, &layout_, seq_lens_dev_, weights_, weights_stride_,
+                               nullptr, budget, sinks, recent, bound_ws_, bound_ws_bytes_, batch_, heads_, dim_, (int32_t)seq_pos, stream);
+    if (rc != HS_OK) return from_abi(rc);
+    copy_upto_ = -1;  // the prompt copy holds the tokens where they were
+    weights_dirty_ = std::max(weights_dirty_, seq_pos);
+    seq_pos = (size_t)budget;
+    return {};
+}
+
 Status LayerKVCache::update(const void *new_keys, const void *new_values, int dtype, int32_t batch, int32_t seq_len,
                             int32_t heads, int32_t dim, size_t start_pos, hs_stream_t stream) {
     if (quant_type_ == KVQuantType::None)
@@ -114,6 +204,8 @@ Status LayerKVCache::update(const void *new_keys, const void *new_values, int dt
     }
     if (Status s = ensure_storage(batch, heads, dim); !s.ok()) return s;
     copy_upto_ = -1;  // tokens written here are not in the prompt copy
+    weights_dirty_ = std::max(weights_dirty_, seq_pos);
+    if (Status s = clean_weights(start_pos, stream); !s.ok()) return s;
     int rc;
     if (quant_type_ == KVQuantType::Fp8) {
         if (start_pos == 0) {  // fresh prompt: calibrate the per-(sequence, head) scales on it
@@ -156,6 +248,12 @@ Status LayerKVCache::decode_attention(const void *q, void *out, int32_t hq, floa
     KVView v;
     if (Status s = get(&v); !s.ok()) return s;
     if (Status s = ensure_scratch(hq, batch_, stream); !s.ok()) return s;
+    if (track_) {
+        if (Status s = ensure_weights(hs_decode_weights_workspace_bytes(batch_, hq, heads_, dim_, (int32_t)max_seq_len), stream); !s.ok()) return s;
+        return from_abi(hs_decode_step_weights(quant_type_ == KVQuantType::Fp8, q, nullptr, nullptr, HS_BF16, k_codes_, v_codes_, k_scales_,
+                                               v_scales_, &layout_, seq_lens_dev_, out, weights_, weights_, weights_stride_, bound_ws_,
+                                               bound_ws_bytes_, batch_, hq, heads_, dim_, (int32_t)seq_pos, scale, stream));
+    }
     int rc = quant_type_ == KVQuantType::Fp8
                  ? hs_decode_attn_fp8(q, (const uint8_t *)k_codes_, (const uint8_t *)v_codes_, k_scales_, v_scales_, &layout_,
                                       seq_lens_dev_, out, workspace_, workspace_bytes_, batch_, hq, heads_, dim_, (int32_t)seq_pos, scale, stream)
@@ -176,7 +274,15 @@ Status LayerKVCache::decode_step(const void *q, const void *k_new, const void *v
     seq_pos += 1;  // the entry point writes the new token at seq_pos - 1 and attends seq_pos tokens
     Status s = ensure_scratch(hq, batch_, stream);
     int rc = HS_OK;
-    if (s.ok()) {
+    if (s.ok() && track_) {
+        if (!k_new || !v_new) s = err(HS_ERR_INVALID_ARGUMENT, "null buffer");
+        if (s.ok()) s = ensure_weights(hs_decode_weights_workspace_bytes(batch_, hq, heads_, dim_, (int32_t)max_seq_len), stream);
+        if (s.ok()) s = clean_weights(seq_pos - 1, stream);
+        if (s.ok())
+            s = from_abi(hs_decode_step_weights(quant_type_ == KVQuantType::Fp8, q, k_new, v_new, dtype, k_codes_, v_codes_, k_scales_, v_scales_,
+                                                &layout_, seq_lens_dev_, out, weights_, weights_, weights_stride_, bound_ws_, bound_ws_bytes_,
+                                                batch_, hq, heads_, dim_, (int32_t)seq_pos, scale, stream));
+    } else if (s.ok()) {
         rc = quant_type_ == KVQuantType::Fp8
                  ? hs_decode_step_fp8(q, k_new, v_new, dtype, (uint8_t *)k_codes_, (uint8_t *)v_codes_, k_scales_, v_scales_, &layout_,
                                       seq_lens_dev_, out, workspace_, workspace_bytes_, batch_, hq, heads_, dim_, (int32_t)seq_pos, scale, stream)
@@ -202,8 +308,15 @@ Status LayerKVCache::prefill(const void *q, const void *new_keys, const void *ne
     }
     if (start_pos > seq_pos) return err(HS_ERR_INVALID_ARGUMENT, "start_pos is past the cached tokens");
     if (Status s = ensure_storage(batch, heads, dim); !s.ok()) return s;
+    weights_dirty_ = std::max(weights_dirty_, seq_pos);
+    if (track_) {
+        const size_t ws = hs_attn_weights_workspace_bytes(batch, seq_len, hq, heads, dim, (int32_t)end_pos);
+        if (Status s = ensure_weights(ws, stream); !s.ok()) return s;
+    }
+    if (Status s = clean_weights(start_pos, stream); !s.ok()) return s;
     int rc;
     hs_kv_layout lay = layout_;
+    lay.prefill_window = window_;
     bool with_copy = false;
     if (prompt_tokens_ > 0) {
         // key-split workspace: sized for the longest chunk seen (grows like the decode workspace)
@@ -254,6 +367,11 @@ Status LayerKVCache::prefill(const void *q, const void *new_keys, const void *ne
     copy_upto_ = rc == HS_OK && with_copy ? (int64_t)end_pos : -1;
     if (rc != HS_OK) return from_abi(rc);
     seq_pos = end_pos;
+    if (track_ && seq_len > 0) {
+        rc = hs_attn_weights(quant_type_ == KVQuantType::Fp8, q, k_codes_, k_scales_, &lay, nullptr, (int32_t)start_pos, weights_, weights_,
+                             weights_stride_, bound_ws_, bound_ws_bytes_, batch, seq_len, hq, heads, dim, (int32_t)end_pos, scale, stream);
+        if (rc != HS_OK) return from_abi(rc);
+    }
     return {};
 }
 
@@ -266,10 +384,13 @@ void LayerKVCache::clear() {
 // quantized storage instead because its blockwise codes straddle tokens, kv_cache.rs:1716-1720).
 void LayerKVCache::truncate_to(size_t pos) {
     if (pos >= seq_pos) return;
+    weights_dirty_ = std::max(weights_dirty_, seq_pos);
     seq_pos = pos;
     copy_upto_ = -1;  // (a prompt that continues from here starts its copy again at position 0 only)
 }
 
-size_t LayerKVCache::memory_usage() const { return k_codes_ ? bytes_ : 0; }
+size_t LayerKVCache::memory_usage() const {
+    return k_codes_ ? bytes_ + (weights_ ? (size_t)batch_ * heads_ * weights_stride_ * sizeof(float) : 0) : 0;
+}
 
 }  // namespace hs

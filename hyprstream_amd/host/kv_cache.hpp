@@ -82,6 +82,18 @@ class LayerKVCache {
     void drop_prompt_scratch();
     bool prompt_copy_active() const { return copy_upto_ >= 0; }  // for tests: the next chunk would read the copy
 
+    // Attention of this layer sees the last `window` cached tokens and the first `sinks` ones (prefill and decode; 0 = all).
+    Status set_window(int32_t window, int32_t sinks);
+    // Count the attention every cached token receives, from here on: decode_attention, decode_step and prefill then add
+    // their softmax weights (summed over queries and over the heads of a group) to fp32 rows [batch, num_kv_heads, .].
+    // A token starts at zero when it is cached; off frees the rows.
+    Status track_weights(bool on);
+    Status get_weights(float *out, hs_stream_t stream = nullptr) const;  // [batch, num_kv_heads, seq_pos]
+    // Keep `budget` tokens per (sequence, kv-head): the first `sinks`, the last `recent`, and the heaviest of those between
+    // (without tracking: the newest).  seq_pos becomes min(seq_pos, budget); keys keep the rotation they were cached with, so
+    // callers rotate later tokens by their true position.
+    Status evict(int32_t budget, int32_t sinks, int32_t recent, hs_stream_t stream = nullptr);
+
     void clear();
     void truncate_to(size_t pos);
     bool is_initialized() const { return k_codes_ != nullptr && seq_pos > 0; }
@@ -94,6 +106,8 @@ class LayerKVCache {
   private:
     Status ensure_storage(int32_t batch, int32_t num_kv_heads, int32_t head_dim);
     Status ensure_scratch(int32_t num_q_heads, int32_t batch, hs_stream_t stream);
+    Status ensure_weights(size_t workspace_bytes, hs_stream_t stream);
+    Status clean_weights(size_t from, hs_stream_t stream);
     void release();
 
     KVQuantType quant_type_;
@@ -105,6 +119,14 @@ class LayerKVCache {
     hs_kv_layout layout_{};
     int32_t batch_ = 0, heads_ = 0, dim_ = 0;
     size_t bytes_ = 0;
+    // bounded cache (set_window, track_weights, evict)
+    int32_t window_ = 0, sinks_ = 0;
+    bool track_ = false;
+    float *weights_ = nullptr;       // [batch, heads, weights_stride_]; zero from seq_pos on, but for [seq_pos, weights_dirty_)
+    int64_t weights_stride_ = 0;
+    size_t weights_dirty_ = 0;
+    void *bound_ws_ = nullptr;       // workspace of the weights' and the eviction's calls
+    size_t bound_ws_bytes_ = 0;
     // prompt scratch (enable_prompt_scratch)
     size_t prompt_tokens_ = 0;       // 0 = not enabled
     void *split_ws_ = nullptr, *copy_ = nullptr;

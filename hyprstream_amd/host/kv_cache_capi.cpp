@@ -80,6 +80,17 @@ int hs_cache_prefill(hs_cache *c, const void *q, const void *k, const void *v, v
     return c->done(c->cache.prefill(q, k, v, out, batch, seq_len, hq, heads, dim, (size_t)start_pos, scale, stream));
 }
 
+int hs_cache_set_window(hs_cache *c, int32_t window, int32_t sinks) {
+    return c ? c->done(c->cache.set_window(window, sinks)) : HS_ERR_INVALID_ARGUMENT;
+}
+int hs_cache_track_weights(hs_cache *c, int on) { return c ? c->done(c->cache.track_weights(on != 0)) : HS_ERR_INVALID_ARGUMENT; }
+int hs_cache_get_weights(hs_cache *c, float *weights_out, hs_stream_t stream) {
+    return c ? c->done(c->cache.get_weights(weights_out, stream)) : HS_ERR_INVALID_ARGUMENT;
+}
+int hs_cache_evict(hs_cache *c, int32_t budget, int32_t sinks, int32_t recent, hs_stream_t stream) {
+    return c ? c->done(c->cache.evict(budget, sinks, recent, stream)) : HS_ERR_INVALID_ARGUMENT;
+}
+
 void hs_cache_enable_prompt_scratch(hs_cache *c, int64_t max_prompt_tokens) {
     if (c && max_prompt_tokens >= 0) c->cache.enable_prompt_scratch((size_t)max_prompt_tokens);
 }

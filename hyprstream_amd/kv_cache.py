@@ -17,7 +17,7 @@ EXPORTS = [
     "hs_cache_get_view", "hs_cache_seq_pos", "hs_cache_max_seq_len", "hs_cache_clear", "hs_cache_truncate_to",
     "hs_cache_is_initialized", "hs_cache_memory_usage", "hs_cache_quant_type", "hs_cache_decode_attention",
     "hs_cache_decode_step", "hs_cache_prefill", "hs_cache_enable_prompt_scratch", "hs_cache_drop_prompt_scratch",
-    "hs_cache_prompt_copy_active", "hs_paged_cache_prefill", "hs_kv_quant_canonical_str",
+    "hs_cache_prompt_copy_active", "hs_cache_set_window", "hs_cache_track_weights", "hs_cache_get_weights", "hs_cache_evict", "hs_paged_cache_prefill", "hs_kv_quant_canonical_str",
     "hs_pool_create", "hs_pool_create_format", "hs_pool_quant_type", "hs_pool_destroy", "hs_pool_last_error", "hs_pool_allocate", "hs_pool_free", "hs_pool_owner_of",
     "hs_pool_used_blocks", "hs_pool_free_block_count", "hs_pool_total_blocks", "hs_pool_used_memory",
     "hs_paged_cache_create", "hs_paged_cache_destroy", "hs_paged_cache_last_error", "hs_paged_cache_update",
@@ -181,6 +181,27 @@ class LayerKVCache(_Handle):
                                            k.shape[2], D, ctypes.c_int64(start_pos), ctypes.c_float(softmax_scale),
                                            hb._stream()))
         return out
+
+    def set_window(self, window, sinks=0):
+        """Attention of this layer sees the last `window` cached tokens (0 = all) and the first `sinks` ones."""
+        self._check(lib().hs_cache_set_window(self._h, ctypes.c_int32(window), ctypes.c_int32(sinks)))
+
+    def track_weights(self, on=True):
+        """Count the attention every cached token receives from here on."""
+        self._check(lib().hs_cache_track_weights(self._h, int(on)))
+
+    def weights(self):
+        """The accumulated weights, fp32 [B, Hkv, seq_pos]."""
+        import torch
+        B, H = ctypes.c_int32(), ctypes.c_int32()
+        self._check(lib().hs_cache_get_view(self._h, None, None, None, None, None, ctypes.byref(B), ctypes.byref(H), None))
+        w = torch.empty(B.value, H.value, self.seq_pos, dtype=torch.float32, device="cuda")
+        self._check(lib().hs_cache_get_weights(self._h, hb._ptr(w), hb._stream()))
+        return w
+
+    def evict(self, budget, sinks=0, recent=0):
+        """Keep `budget` tokens per (sequence, kv-head): the first `sinks`, the last `recent`, the heaviest between."""
+        self._check(lib().hs_cache_evict(self._h, ctypes.c_int32(budget), ctypes.c_int32(sinks), ctypes.c_int32(recent), hb._stream()))
 
     def enable_prompt_scratch(self, max_prompt_tokens):
         """Opt in to the key split of small prefill calls and to the bf16 copy of the prompt (hs_cache_enable_prompt_scratch)."""

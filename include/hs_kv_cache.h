@@ -100,6 +100,21 @@ HS_API int hs_cache_prefill(hs_cache *c, const void *q, const void *new_keys, co
                             int32_t batch, int32_t seq_len, int32_t num_q_heads, int32_t num_kv_heads,
                             int32_t head_dim, int64_t start_pos, float softmax_scale, hs_stream_t stream);
 
+/* ---- a bounded cache (no counterpart in the reference, whose caches grow to max_seq_len and then fail) --------------
+ * hs_cache_set_window: this layer's attention sees the last `window` cached tokens and the first `sinks` ones, in prefill
+ *   and decode (hs_kv_layout.prefill_window, decode_window, attn_sinks); 0 = everything.
+ * hs_cache_track_weights: from here on every attention call through the cache adds its softmax weights, summed over queries
+ *   and over the query heads of a kv-head, to one fp32 entry per cached token (hs_decode_step_weights, hs_attn_weights).  A
+ *   token starts at zero when it is cached; 0 stops and frees the entries.
+ * hs_cache_get_weights: the entries as dense [batch, num_kv_heads, seq_pos], copied on `stream`.
+ * hs_cache_evict: keeps `budget` tokens per (sequence, kv-head) -- the first `sinks`, the last `recent` and the heaviest of
+ *   those between; without tracking the first `sinks` and the newest -- in place (hs_kv_evict).  seq_pos becomes
+ *   min(seq_pos, budget).  Keys keep their rotation: rotate later tokens by their true position, not by seq_pos. */
+HS_API int hs_cache_set_window(hs_cache *c, int32_t window, int32_t sinks);
+HS_API int hs_cache_track_weights(hs_cache *c, int on);
+HS_API int hs_cache_get_weights(hs_cache *c, float *weights_out, hs_stream_t stream);
+HS_API int hs_cache_evict(hs_cache *c, int32_t budget, int32_t sinks, int32_t recent, hs_stream_t stream);
+
 /* Opt in to faster prompts through hs_cache_prefill (no counterpart in the reference, whose get() dequantizes the whole
  * cache on every call, kv_cache.rs:1493-1560).  After this call prefill offers the library a key-split workspace (a
  * chunk of ONE sequence is too few query tiles for the GPU: the keys of a tile are then split over workgroups) and,
