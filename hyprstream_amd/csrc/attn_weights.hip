@@ -361,6 +361,7 @@ __global__ __launch_bounds__(kWThreads, 2) void weights_stats_kernel(WeightsArgs
         if (lq != 0 || c >= a.lse_stride) continue;
         if (a.key_chunks == 1) {
             a.lse[(int64_t)unit * a.lse_stride + c] = L == 0.0f ? INFINITY : M + __builtin_amdgcn_logf(L);
+            if (NB == 1) a.lse[(int64_t)unit * a.lse_stride + c + WGC] = INFINITY;  // the row's other half, without columns
         } else if (c < a.cols) {
             float *ml = a.part_ml + (((int64_t)unit * a.key_chunks + chunk) * a.cols + c) * 2;
             ml[0] = M;
@@ -431,7 +432,7 @@ __global__ __launch_bounds__(kWThreads, 2) void weights_columns_kernel(WeightsAr
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
         sum[u] = before[u] = (float4v){0.f, 0.f, 0.f, 0.f};
-        if (a.segments == 1 && a.in && li == 0) before[u] = *(const float4v *)(a.in + (int64_t)unit * a.stride + min(wk0 + 16 * u + 4 * lq, (int)a.stride - 4));
+        if (a.segments == 1 && a.in && li == 0) before[u] = *(const float4v *)(a.in + (int64_t)unit * a.stride + min((int64_t)(wk0 + 16 * u + 4 * lq), a.stride - 4));
     }
     if (c_lo < c_hi) {
         // ---- columns, kCStep a step: copy i of this thread is piece (x % CPR) of the tile's column x / CPR, x = tid + 512 i.
@@ -444,7 +445,7 @@ __global__ __launch_bounds__(kWThreads, 2) void weights_columns_kernel(WeightsAr
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) {
             const int x = tid + kWThreads * i, c = x / CPR;
-            off[i] = (uint32_t)(((c / a.G) * a.Hq + c % a.G) * D * 2 + 16 * ((x % CPR) ^ (c & SWZ)));
+            off[i] = (uint32_t)((c / a.G) * a.Hq + c % a.G) * (D * 2) + 16 * ((x % CPR) ^ (c & SWZ));
         }
         auto fetch = [&](int c0, int buf) {
             uint8_t *dst = sm + buf * kTile + 1024 * wave;
@@ -609,7 +610,7 @@ static WeightsPlan plan_weights(int B, int S, int Hq, int Hkv, int D, int max_se
     WeightsPlan p;
     const int64_t units = (int64_t)B * Hkv;
     p.cols = (int64_t)S * (Hq / Hkv);
-    // a wavefront holds 32 columns; sixteen at head_dim 256 (registers) and when all columns fit one workgroup that way
+    // a wavefront holds 64 columns; 32 at head_dim 256 (registers), fewer when all columns fit one workgroup that way
     p.nb = p.cols <= 64 ? 1 : p.cols <= 128 || D == 256 ? 2 : 4;
     const int wg_cols = kWThreads / 4 * p.nb, wg_keys = kWThreads / 4 * (D == 256 ? 2 : 4);
     p.col_blocks = (p.cols + wg_cols - 1) / wg_cols;

@@ -351,7 +351,7 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
     const int n = a.info[2 * row], i0 = blockIdx.x * kMoveTokens;
     if (blockIdx.x == 0 && h == 0 && tid == 0) a.seq_lens_out[b] = n;
     if (blockIdx.x == 0 && a.fp8 && tid < 2) (tid ? a.vso : a.kso)[row] = (tid ? a.vs : a.ks)[row];
-    finish_rows(a, row, n, i0, i0 + kMoveTokens, tid, 256);
+    finish_rows(a, row, n, i0, (int)min((int64_t)i0 + kMoveTokens, (int64_t)a.finish), tid, 256);
     if (i0 < n) move_tile<D, 256, kMoveTokens>(a, row, b, h, n, i0, tid);
 }
 
@@ -519,7 +519,7 @@ int hs_kv_evict(int fmt_fp8, const void *k_codes, const void *v_codes, const flo
         else if (D == 128) evict_inplace_kernel<128><<<grid, 1024, 0, st>>>(a);
         else evict_inplace_kernel<256><<<grid, 1024, 0, st>>>(a);
     } else {
-        const dim3 grid((a.finish + kMoveTokens - 1) / kMoveTokens, Hkv, B);
+        const dim3 grid((unsigned)(((int64_t)a.finish + kMoveTokens - 1) / kMoveTokens), Hkv, B);
         if (D == 64) evict_move_kernel<64><<<grid, 256, 0, st>>>(a);
         else if (D == 128) evict_move_kernel<128><<<grid, 256, 0, st>>>(a);
         else evict_move_kernel<256><<<grid, 256, 0, st>>>(a);

@@ -126,6 +126,24 @@ def test_prompt_weights(case):
     assert torch.equal(torch.where(first == -7.0, w, first), w)
 
 
+@pytest.mark.parametrize("S,at,Hq,Hkv,D,T", [(1, 100, 4, 1, 128, 400), (7, 0, 8, 1, 64, 500), (16, 30, 8, 2, 128, 512), (3, 5, 4, 4, 256, 2000),
+                                             (20, 60, 6, 1, 128, 1500)])
+def test_prompt_weights_of_a_cache_with_room(S, at, Hq, Hkv, D, T):
+    """Few queries, max_seq_len far behind the last one."""
+    c = Cache(4350 + T, 1, Hkv, T, D)
+    q = bf16_randn(4351, 1, S, Hq, D)
+    n = at + S
+    ws = torch.full((hb.attn_weights_workspace_bytes(1, S, Hq, Hkv, D, T),), 0xFF, dtype=torch.uint8, device=DEV)
+    _, add, _, bound = attention(f64(q[0]), c.K[0, :n], None, at + np.arange(S), 0, 0, D ** -0.5)
+    for fill in (0xFF, 0):  # whatever the workspace held
+        ws.fill_(fill)
+        wo = torch.full((1, Hkv, T), -7.0, device=DEV)
+        hb.attn_weights(q, c.tensors[0], c.tensors[2], c.layout, None, wo, ws, Hkv, T, D ** -0.5, start_pos=at)
+        got = f64(wo)[0]
+        assert (got[:, n:] == -7.0).all()
+        assert (np.abs(got[:, :n] - add) <= weight_tolerance(add, add, bound, D, S * Hq // Hkv)).all()
+
+
 @pytest.mark.parametrize("D,fp8", [(128, False), (64, True)])
 def test_prompt_weights_at_positions(D, fp8):
     """Rows at positions of their own; queries outside [0, max_seq_len) count nothing, NaN in their place or in tokens
