@@ -269,6 +269,10 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
                 resolve(a.va, b, 0, unit, slot);
                 n = min(min(H, 64), a.va.capacity_tokens - slot);
                 rv = a.vs[unit * a.va.scale_stride_seq + (int64_t)kvh * a.va.scale_stride_head + slot + min(lane, n - 1)];
+                if (kWin) {  // (a token the window hides may hold anything)
+                    rk = rk < 3.0e38f ? rk : 0.0f;
+                    rv = rv < 3.0e38f ? rv : 0.0f;
+                }
                 rk = wave_max(rk);
                 rv = wave_max(rv);
             }
@@ -426,6 +430,12 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
                 if (krow > last) fk = 0.0f;
                 if (vkey > last) fv0 = 0.0f;
                 if (vkey + 1 > last) fv1 = 0.0f;
+            }
+            if (kWin && step * kHStep < H + wg_lo) {  // so do tokens that no query of the workgroup sees
+                const int sink_end = a.sinks - step * kHStep, first = H + wg_lo - step * kHStep;
+                if (krow >= sink_end && krow < first) fk = 0.0f;
+                if (vkey >= sink_end && vkey < first) fv0 = 0.0f;
+                if (vkey + 1 >= sink_end && vkey + 1 < first) fv1 = 0.0f;
             }
             // largest operand: 127 * scale (int8), 1.75 * 256 * scale (fp8), scale relative to the head's reference:
             // rows more than 2^11 above it saturate here instead of overflowing

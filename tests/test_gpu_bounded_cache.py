@@ -378,3 +378,38 @@ def test_mirror_refusals():
         cache.weights()
     cache.evict(30)
     assert cache.seq_pos == 20
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_scales_of_hidden_tokens_do_not_matter(D, bad):
+    """Scales that are no numbers in tokens that the window hides: every output keeps its bits, but for prefill's.  Its
+    operands are fp16 relative to a power of two that the first tokens' scales choose, hidden ones among them: without
+    those it may be another power.  Then only q elements that fp16 holds as subnormals round elsewhere, by at most 2^-25
+    each; history operands are below 127/4 < 2^5, so a score moves by at most D 2^-20 (log2 units), a weight by twice
+    ln 2 times that relative to itself, the output by as much of the largest |v|, and bf16 may round to the neighbour."""
+    B, Hq, Hkv, T, S, window, sinks = 2, 8, 2, 500, 40, 101, 5
+    q, qs = bf16_randn(6900, B, Hq, D), bf16_randn(6901, B, S, Hq, D)
+    kn, vn = bf16_randn(6902, B, S, Hkv, D), bf16_randn(6903, B, S, Hkv, D)
+    seq = torch.full((B,), T, dtype=torch.int32, device=DEV)
+    ws = _space(max(hb.decode_weights_workspace_bytes(B, Hq, Hkv, D, T + S), hb.attn_weights_workspace_bytes(B, S, Hq, Hkv, D, T + S)))
+    got = []
+    for fill in (None, bad):
+        c = Cache(6904, B, Hkv, T + S, D)
+        outs = [torch.empty(B, Hq, D, dtype=torch.bfloat16, device=DEV) for _ in range(2)] + [torch.empty_like(qs)]
+        w = [torch.zeros(B, Hkv, T + S, device=DEV) for _ in range(2)]
+        if fill is not None:  # hidden from the query at T - 1 and from every later one
+            for t in c.tensors[2:]:
+                t[:, :, sinks:T - window] = fill
+        hb.decode_attn(q, *c.tensors, c.layout, seq, outs[0], ws, Hkv, T, 0.1, window=window, sinks=sinks)
+        hb.decode_step_weights(q, None, None, *c.tensors, c.layout, seq, outs[1], None, w[0], ws, Hkv, T, 0.1, window=window, sinks=sinks)
+        hb.prefill_attn(qs, kn, vn, *c.tensors, c.layout, T, outs[2], 0.1, window=window, sinks=sinks)
+        hb.attn_weights(qs, c.tensors[0], c.tensors[2], c.layout, None, w[1], ws, Hkv, T + S, 0.1, start_pos=T, window=window, sinks=sinks)
+        got.append(outs + w)
+    for i, (a, b) in enumerate(zip(*got)):
+        assert torch.isfinite(a.float()).all() and torch.isfinite(b.float()).all(), i
+        if i == 2:
+            x, y, vmax = f64(a), f64(b), vn.abs().max().item() + np.abs(c.V[:, :sinks]).max() + np.abs(c.V[:, T - window:T]).max()
+            assert (np.abs(x - y) <= 2.0 ** -7 * np.maximum(np.abs(x), np.abs(y)) + 2 * np.log(2) * D * 2.0 ** -20 * vmax).all()
+        else:
+            assert torch.equal(a, b), i
