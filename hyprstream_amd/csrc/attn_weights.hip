@@ -6,7 +6,8 @@
 //
 // lse_c is needed before the first p and takes all of s, so s is computed twice: weights_stats_kernel walks the keys for
 // a block of columns and leaves (m, l) per column, weights_columns_kernel walks the columns for a block of keys and adds
-// up.  Storing p in between instead would move S x T values per query head.  Both products run on the matrix cores with
+// up.  (weights_narrow_kernel does both where all columns fit a wavefront.)  Storing p in between instead would move S x T
+// values per query head.  Both products run on the matrix cores with
 // exact operands (the result is an fp32 tensor, and a rounded operand would show in it): codes are integers (int8) or
 // short floats (e4m3fn) that fp16 and bf16 hold exactly, q is bf16.  Each kernel keeps its stationary side in registers
 // and converts only there or once per workgroup: columns as fp16 in the first (the streamed codes take one byte permute
@@ -361,9 +362,251 @@ __global__ __launch_bounds__(kWThreads, 2) void weights_stats_kernel(WeightsArgs
         if (lq != 0 || c >= a.lse_stride) continue;
         if (a.key_chunks == 1) {
             a.lse[(int64_t)unit * a.lse_stride + c] = L == 0.0f ? INFINITY : M + __builtin_amdgcn_logf(L);
-            if (NB == 1) a.lse[(int64_t)unit * a.lse_stride + c + WGC] = INFINITY;  // the row's other half, without columns
         } else if (c < a.cols) {
             float *ml = a.part_ml + (((int64_t)unit * a.key_chunks + chunk) * a.cols + c) * 2;
+            ml[0] = M;
+            ml[1] = L;
+        }
+    }
+}
+
+// Few columns (an observation window of the last queries, or single tokens): a wavefront holds all of them as B operands and
+// streams keys from memory straight into A operands, sixteen at a time, two steps ahead; no barrier in the loop.  Against the
+// wide kernels (us a call): one query on 64 x 8 rows of 8192 keys 443 -> 224 (1.07 GB of codes read in the two passes: 4.8
+// TB/s), one on 8 x 32768 39.6 -> 25, 32 queries (128 columns) there 49 -> 38.  At 128 columns the vector pipe bounds it:
+// about 200 instructions, 32 exponentials and 32 products per 16 keys do not overlap further with two wavefronts a SIMD.
+// Operand j of a lane is d = (D/4) lq + 8 j ..: a lane's codes of a key lie together, and q is used as it lies (bf16).
+// COLUMNS false: (m, l) of the columns over a chunk of keys; true: the weights of a chunk's keys, lse given.
+template <int D, bool FP8, int NB, bool COLUMNS>
+__global__ __launch_bounds__(kWThreads, 2) void weights_narrow_kernel(WeightsArgs a) {
+    constexpr int KG = D / 32, LOADS = D / 64;  // 16-byte loads of a lane per key
+    constexpr float kOver = 8.0f, kFar = 64.0f;  // as in weights_stats_kernel
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int li = lane & 15, lq = lane >> 4;
+    const int units = a.B * a.Hkv, unit = blockIdx.x % units, chunk = blockIdx.x / units;
+    const int b = unit / a.Hkv, h = unit % a.Hkv;
+    const int pos0 = first_pos(a, b), T = key_count(a, pos0);
+    const int p_first = max(pos0, 0), p_last = T - 1;  // of the queries that see anything
+    const int c_lo = chunk * a.chunk_tokens, c_hi = min(c_lo + a.chunk_tokens, T);
+    const int s_hi = c_hi > c_lo ? (c_hi + kWStep - 1) / kWStep : 0;
+    const int sink_steps = a.window ? (a.sinks + kWStep - 1) / kWStep : 0;
+    const int win_step = a.window ? max(0, p_first - a.window + 1) / kWStep : 0;
+    auto gap = [&](int st) { return a.window && st >= sink_steps && st < win_step; };  // nobody sees a key of the step
+    // without a sum to write (or with the one that is there already) such steps are left out
+    const bool skips = !COLUMNS || a.in == a.out;
+    auto next_step = [&](int st) { return skips && gap(st) ? win_step : st; };
+    int st = next_step(c_lo / kWStep), nst = next_step(st + 1);
+    if (COLUMNS && st >= s_hi) return;
+
+    u32x4 raw[2][LOADS];
+    float rawsc[2][4];
+    float4v before[2];
+    // Always as many loads, whatever the step is (behind the end the last one again, in the gap the one behind it): only then
+    // is a wait for the older of two loads in flight not a wait for both.
+    const float *in = a.in ? a.in : a.out;
+    auto load = [&](int step, auto slot_tag) {
+        constexpr int kSlot = decltype(slot_tag)::value;
+        step = min(step, s_hi - 1);
+        if (COLUMNS) {
+            const int t = step * kWStep + 16 * wave + 4 * lq;
+            before[kSlot] = *(const float4v *)(in + (int64_t)unit * a.stride + min((int64_t)t, a.stride - 4));
+            if (gap(step)) step = min(win_step, s_hi - 1);
+        }
+        const int t0 = step * kWStep, last = T - 1 - t0;
+        const KeyBase k = key_base(a, b, h, t0, D, FP8);
+        const uint8_t *src = k.codes + (uint32_t)(min(16 * wave + li, last) * D + D / 4 * lq);
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) raw[kSlot][i] = *(const u32x4 *)(src + 16 * i);
+        if (!FP8) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) rawsc[kSlot][r] = k.scales[min(16 * wave + 4 * lq + r, last)];
+        }
+    };
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        const float head_scale = FP8 ? a.ks[(int64_t)b * a.Hkv + h] : 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) rawsc[s][r] = head_scale;
+    }
+    if (s_hi > 0) {
+        load(st, std::integral_constant<int, 0>{});
+        load(nst, std::integral_constant<int, 1>{});
+    }
+    // ---- columns: block nb, column li.  One that sees nothing (no query, or none inside [0, max_seq_len)) is zero.  They come
+    //      through LDS (16-byte piece pc of column c at piece pc ^ c, modulo 16): read by every wavefront for itself, 64 MB
+    //      from L2 at 512 workgroups, the columns took 8 us of a kernel of 24.
+    constexpr int CPR = D / 8, SWZ = CPR < 16 ? CPR - 1 : 15;
+    __shared__ __attribute__((aligned(16))) uint8_t sm_q[16 * NB * D * 2];
+#pragma unroll
+    for (int i = 0; i < 16 * NB * CPR / kWThreads; ++i) {
+        const int x = tid + kWThreads * i, c = x / CPR, cc = min(c, a.cols - 1), s = cc / a.G;
+        copy16_to_lds(a.q + (((int64_t)b * a.S + s) * a.Hq + h * a.G + cc - s * a.G) * D + 8 * ((x % CPR) ^ (c & SWZ)), sm_q + 16 * (kWThreads * i + 64 * wave));
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    bf16x8 qop[NB][KG];
+    int pos[NB];
+    float m[NB], l[NB], sum[4];  // COLUMNS: m = lse
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        const int c = 16 * nb + li, p = pos0 + min(c, a.cols - 1) / a.G;
+        pos[nb] = c < a.cols && p < a.max_seq_len ? max(p, -1) : -1;
+#pragma unroll
+        for (int j = 0; j < KG; ++j) {
+            const u32x4 w = *(const u32x4 *)(sm_q + (c * CPR + ((KG * lq + j) ^ (c & SWZ))) * 16) & (uint32_t)~(pos[nb] >> 31);
+            qop[nb][j] = pack_bf16x8(w[0], w[1], w[2], w[3]);
+        }
+        m[nb] = COLUMNS ? a.lse[(int64_t)unit * a.lse_stride + 16 * nb + li] : 0.0f;
+        l[nb] = 0.0f;
+    }
+    // the loads above end here: a wait for them inside the loop would be a wait for the keys of the steps ahead as well
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+        asm volatile("" : "+v"(m[nb]));
+#pragma unroll
+        for (int j = 0; j < KG; ++j) asm volatile("" : "+v"(qop[nb][j]));
+    }
+    bool force = true;  // some column has no bound yet
+    auto body = [&](auto slot_tag) {
+        constexpr int kSlot = decltype(slot_tag)::value;
+        const int t0 = st * kWStep + 16 * wave;  // this wavefront's keys
+        bf16x8 kop[KG];
+        float sk[4];
+        // (the codes are unpacked here: carried through the loop as bytes they take four times the registers)
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) asm volatile("" : "+v"(raw[kSlot][i]));
+#pragma unroll
+        for (int j = 0; j < KG; ++j) kop[j] = codes_to_bf16<FP8>(raw[kSlot][j / 2][2 * (j & 1)], raw[kSlot][j / 2][2 * (j & 1) + 1]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            sk[r] = rawsc[kSlot][r] * a.scale_log2e;
+            sum[r] = 0.0f;
+        }
+        const float4v start = before[kSlot];
+        const int after = next_step(nst + 1);
+        load(after, slot_tag);
+        const bool edge = t0 + 15 > p_first || (a.window && t0 <= p_last - a.window);
+        // The products of block nb among the weights of block nb - 1, each added up one weight later, in a pinned order.
+        float4v acc[2];
+        auto products = [&](int nb, int j) { acc[nb & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kop[j], qop[nb][j], j == 0 ? (float4v){0.f, 0.f, 0.f, 0.f} : acc[nb & 1], 0, 0, 0); };
+        auto blocks = [&](auto look, auto add) {
+            float pend = 0.0f;
+#pragma unroll
+            for (int nb = 0; nb <= NB; ++nb) {
+#pragma unroll
+                for (int j = 0; j < KG; ++j) {
+                    if (nb < NB) products(nb, j);
+                    if (nb > 0) {
+#pragma unroll
+                        for (int r = j * 4 / KG; r < (j + 1) * 4 / KG; ++r) {
+                            const int i = 4 * (nb - 1) + r;
+                            if (i > 0) add((i - 1) / 4, (i - 1) % 4, pend);
+                            const float x = acc[(nb - 1) & 1][r] * sk[r] - m[nb - 1];
+                            look(x);
+                            pend = __builtin_amdgcn_exp2f(x);
+                        }
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            add(NB - 1, 3, pend);
+        };
+        if (t0 < T && !(COLUMNS && gap(st))) {
+            if constexpr (COLUMNS) {
+                auto none = [](float) {};
+                if (edge) blocks(none, [&](int nb, int r, float w) { sum[r] += sees(pos[nb], window_lo(a, pos[nb]), a.sinks, t0 + 4 * lq + r) ? w : 0.0f; });
+                else blocks(none, [&](int, int r, float w) { sum[r] += w; });
+            } else {
+                bool done = false;
+                if (!edge && !force) {  // no comparisons but one: done again with them if a score is far above its bound
+                    float l_old[NB];
+                    int over = INT_MIN, last_x = INT_MIN;
+                    bool second = false;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) l_old[nb] = l[nb];
+                    blocks(
+                        [&](float x) {
+                            if (second) over = max(over, max(last_x, __float_as_int(x)));  // positive floats order like their bits
+                            last_x = __float_as_int(x);
+                            second = !second;
+                        },
+                        [&](int nb, int, float w) { l[nb] += w; });
+                    done = __builtin_amdgcn_ballot_w64(over > __float_as_int(kFar)) == 0;
+                    if (!done) {
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) l[nb] = l_old[nb];
+                    }
+                }
+                if (!done) {
+                    bool open = false;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                        for (int j = 0; j < KG; ++j) products(nb, j);
+                        float e[4], mx = -INFINITY;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            e[r] = acc[nb & 1][r] * sk[r] - m[nb];
+                            if (edge && !sees(pos[nb], window_lo(a, pos[nb]), a.sinks, t0 + 4 * lq + r)) e[r] = -INFINITY;
+                            mx = fmaxf(mx, e[r]);
+                        }
+                        float up = 0.0f;
+                        if (l[nb] == 0.0f) up = mx > -INFINITY ? mx + kOver : 0.0f;  // the column's first keys in this lane
+                        else if (mx > 0.0f) up = mx + kOver;
+                        l[nb] *= __builtin_amdgcn_exp2f(-up);
+                        m[nb] += up;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) l[nb] += __builtin_amdgcn_exp2f(e[r] - up);
+                        open = open || (pos[nb] >= 0 && l[nb] == 0.0f);
+                    }
+                    force = __builtin_amdgcn_ballot_w64(open) != 0;
+                }
+            }
+        }
+        if constexpr (COLUMNS) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum[r] = (a.in ? start[r] : 0.0f) + row_sum(sum[r]);
+            const int t = t0 + 4 * lq;
+            if (li == 0 && t < T) {
+                float *o = a.out + (int64_t)unit * a.stride + t;
+                if (t + 4 <= T) *(float4v *)o = (float4v){sum[0], sum[1], sum[2], sum[3]};
+                else
+                    for (int r = 0; r < 4; ++r)
+                        if (t + r < T) o[r] = sum[r];
+            }
+        }
+        st = nst;
+        nst = after;
+    };
+    while (st < s_hi) {
+        body(std::integral_constant<int, 0>{});
+        if (st >= s_hi) break;
+        body(std::integral_constant<int, 1>{});
+    }
+    if constexpr (!COLUMNS) {
+        // ---- join the four lanes of a column, then the wavefronts
+        __shared__ float sm_m[4][16 * NB], sm_l[4][16 * NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const bool none = l[nb] == 0.0f || pos[nb] < 0;
+            const float mine = none ? -INFINITY : m[nb], M = quad_max(mine);
+            const float L = quad_sum(none ? 0.0f : l[nb] * __builtin_amdgcn_exp2f(mine - M));
+            if (lq == 0) {
+                sm_m[wave][16 * nb + li] = M;
+                sm_l[wave][16 * nb + li] = L;
+            }
+        }
+        __syncthreads();
+        if (tid >= 16 * NB) return;
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_m[w][tid]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) L += sm_m[w][tid] == -INFINITY ? sm_l[w][tid] : sm_l[w][tid] * __builtin_amdgcn_exp2f(sm_m[w][tid] - M);
+        if (a.key_chunks == 1) {
+            a.lse[(int64_t)unit * a.lse_stride + tid] = L == 0.0f ? INFINITY : M + __builtin_amdgcn_logf(L);
+        } else if (tid < a.cols) {
+            float *ml = a.part_ml + (((int64_t)unit * a.key_chunks + chunk) * a.cols + tid) * 2;
             ml[0] = M;
             ml[1] = L;
         }
@@ -600,6 +843,7 @@ int check_weights(const float *in, const float *out, int64_t stride, int max_seq
 
 struct WeightsPlan {
     int64_t cols, col_blocks, key_blocks, lse_stride;
+    bool narrow;
     int nb;  // 16-column blocks per wavefront of the first kernel
     int key_chunks, chunk_tokens, segments;
     int64_t part_stride;
@@ -610,38 +854,53 @@ static WeightsPlan plan_weights(int B, int S, int Hq, int Hkv, int D, int max_se
     WeightsPlan p;
     const int64_t units = (int64_t)B * Hkv;
     p.cols = (int64_t)S * (Hq / Hkv);
-    // a wavefront holds 64 columns; 32 at head_dim 256 (registers), fewer when all columns fit one workgroup that way
-    p.nb = p.cols <= 64 ? 1 : p.cols <= 128 || D == 256 ? 2 : 4;
+    // All columns in the registers of one wavefront (128; 64 at head_dim 256): the narrow kernels.  Else a wavefront of the
+    // first kernel holds 64 columns (32).
+    const int most = D == 256 ? 64 : 128;
+    p.narrow = p.cols <= most;
+    p.nb = !p.narrow ? most / 32 : p.cols <= 32 ? 2 : p.cols <= 64 ? 4 : 8;
     const int wg_cols = kWThreads / 4 * p.nb, wg_keys = kWThreads / 4 * (D == 256 ? 2 : 4);
-    p.col_blocks = (p.cols + wg_cols - 1) / wg_cols;
+    p.col_blocks = p.narrow ? 1 : (p.cols + wg_cols - 1) / wg_cols;
     p.key_blocks = ((int64_t)max_seq_len + wg_keys - 1) / wg_keys;
-    // First kernel: few columns (an observation window) leave most CUs idle unless the keys are split, into chunks of
-    // at least 512 (8 units, 128 columns, 32768 keys, us: 21.8 with chunks of 512, 23.4 with 256, 28.7 with 128).
-    const int64_t want = std::max<int64_t>(1, 1024 / std::max<int64_t>(1, units * p.col_blocks));
-    int64_t ct = ((int64_t)max_seq_len + want - 1) / want;
-    ct = std::max<int64_t>(512, (ct + kWStep - 1) / kWStep * kWStep);
+    // Few columns leave most CUs idle unless the keys are split.  Narrow: 512 workgroups, one round, of at least 128 keys (32
+    // columns x 16 on 8 units, 4096 keys, us a call: 15.0 with 128, 17.5 with 256, 22.7 with 512) and at most 4096 (512 units
+    // x 8192 keys, single queries: 223 us, 246 with one chunk).  Wide: at least 512
+    // keys (256 columns on 8 units, 32768 keys: 70 us, 77 with 256, 71 with 1024).
+    const int64_t want = std::max<int64_t>(1, (p.narrow ? 512 : 1024) / std::max<int64_t>(1, units * p.col_blocks));
+    int64_t ct = (((int64_t)max_seq_len + want - 1) / want + kWStep - 1) / kWStep * kWStep;
+    ct = p.narrow ? std::min<int64_t>(4096, std::max<int64_t>(128, ct)) : std::max<int64_t>(512, ct);
     p.chunk_tokens = (int)std::min<int64_t>(ct, ((int64_t)max_seq_len + kWStep - 1) / kWStep * kWStep);
     p.key_chunks = (int)(((int64_t)max_seq_len + p.chunk_tokens - 1) / p.chunk_tokens);
     // Second kernel: two workgroups are resident on each of 256 CUs, and each of them should come round twice: started in
     // order of their work, long items then meet short ones and the causal triangle evens out (4 x 4096 tokens, 16 key
     // blocks on 32 units, us: 369 with one share of the columns, 305 with two, 308 with four).
     const int64_t items = units * p.key_blocks, steps = (p.cols + kCStepMax - 1) / kCStepMax;
-    p.segments = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(steps, 16), (1024 + items - 1) / items));
+    p.segments = p.narrow ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(steps, 16), (1024 + items - 1) / items));
     p.part_stride = p.key_blocks * wg_keys;
-    p.lse_stride = (p.cols + 127) / 128 * 128;
+    p.lse_stride = p.narrow ? 16 * p.nb : (p.cols + 127) / 128 * 128;
     p.lse_floats = (size_t)(units * p.lse_stride);
     p.ml_floats = p.key_chunks > 1 ? (size_t)units * p.key_chunks * p.cols * 2 : 0;
     p.w_floats = p.segments > 1 ? (size_t)p.segments * units * p.part_stride : 0;
     return p;
 }
 
+template <int D, bool FP8, int NB>
+static void launch_narrow(const WeightsArgs &a, const WeightsPlan &p, hipStream_t st) {
+    const int64_t units = (int64_t)a.B * a.Hkv;
+    weights_narrow_kernel<D, FP8, NB, false><<<(unsigned)(units * p.key_chunks), kWThreads, 0, st>>>(a);
+    if (p.key_chunks > 1) weights_join_kernel<<<(unsigned)((units * p.lse_stride + 15) / 16), 256, 0, st>>>(a);
+    weights_narrow_kernel<D, FP8, NB, true><<<(unsigned)(units * p.key_chunks), kWThreads, 0, st>>>(a);
+}
+
 template <int D, bool FP8>
 static void launch_weights(const WeightsArgs &a, const WeightsPlan &p, hipStream_t st) {
     const int64_t units = (int64_t)a.B * a.Hkv;
-    const unsigned grid = (unsigned)(units * p.key_chunks * p.col_blocks);
-    if (p.nb == 1) weights_stats_kernel<D, FP8, 1><<<grid, kWThreads, 0, st>>>(a);
-    else if (p.nb == 2) weights_stats_kernel<D, FP8, 2><<<grid, kWThreads, 0, st>>>(a);
-    else if constexpr (D < 256) weights_stats_kernel<D, FP8, 4><<<grid, kWThreads, 0, st>>>(a);
+    if (p.narrow) {
+        if (p.nb == 2) return launch_narrow<D, FP8, 2>(a, p, st);
+        if (p.nb == 4) return launch_narrow<D, FP8, 4>(a, p, st);
+        if constexpr (D < 256) return launch_narrow<D, FP8, 8>(a, p, st);
+    }
+    weights_stats_kernel<D, FP8, D == 256 ? 2 : 4><<<(unsigned)(units * p.key_chunks * p.col_blocks), kWThreads, 0, st>>>(a);
     if (p.key_chunks > 1) weights_join_kernel<<<(unsigned)((units * p.lse_stride + 15) / 16), 256, 0, st>>>(a);
     weights_columns_kernel<D, FP8><<<(unsigned)(units * p.segments * p.key_blocks), kWThreads, 0, st>>>(a);
     if (p.segments > 1) weights_sum_kernel<<<dim3((unsigned)((a.max_seq_len + 1023) / 1024), (unsigned)units), 256, 0, st>>>(a);

@@ -126,6 +126,36 @@ def test_prompt_weights(case):
     assert torch.equal(torch.where(first == -7.0, w, first), w)
 
 
+FEW = [  # B, S, start, Hq, Hkv, D, window, sinks, fp8, paged: columns that fit one wavefront
+    (2, 1, 2000, 4, 2, 64, 0, 0, False, 64),
+    (1, 9, 700, 12, 2, 128, 0, 0, True, 64),
+    (3, 16, 1300, 12, 3, 256, 0, 0, False, 0),
+    (1, 16, 999, 8, 2, 256, 333, 70, True, 64),
+    (2, 40, 900, 9, 3, 128, 65, 0, False, 0),
+    (1, 64, 0, 4, 2, 64, 17, 2, False, 0),
+    (1, 21, 3001, 18, 3, 128, 1000, 130, False, 64),
+]
+
+
+@pytest.mark.parametrize("case", FEW, ids=lambda c: "B%d-S%d-at%d-%d/%d-D%d-w%d-s%d-%s%s" % (c[:8] + ("fp8" if c[8] else "int8", "-p%d" % c[9] if c[9] else "")))
+def test_prompt_weights_of_few_queries(case):
+    """From nothing, from other rows and in place; the last token of the cache is never the last position."""
+    B, S, at, Hq, Hkv, D, window, sinks, fp8, paged = case
+    n, T = at + S, at + S + 77
+    c = Cache(4250 + T, B, Hkv, T, D, fp8=fp8, paged=paged)
+    q, w = bf16_randn(4251, B, S, Hq, D), _rows(4252, B, Hkv, T)
+    ws = torch.full((hb.attn_weights_workspace_bytes(B, S, Hq, Hkv, D, T),), 0xFF, dtype=torch.uint8, device=DEV)
+    ref = [attention(f64(q[b]), c.K[b, :n], None, at + np.arange(S), window, sinks, D ** -0.5)[1::2] for b in range(B)]
+    inplace = w.clone()
+    for win, wout in ((None, torch.full_like(w, -7.0)), (w, torch.full_like(w, -7.0)), (inplace, inplace)):
+        hb.attn_weights(q, c.tensors[0], c.tensors[2], c.layout, win, wout, ws, Hkv, T, D ** -0.5, start_pos=at, fp8=fp8, window=window, sinks=sinks)
+        start, got = np.zeros(w.shape) if win is None else f64(w), f64(wout)
+        assert (got[:, :, n:] == (start[:, :, n:] if wout is inplace else -7.0)).all()
+        for b, (add, bound) in enumerate(ref):
+            err = np.abs(got[b, :, :n] - start[b, :, :n] - add)
+            assert (err <= weight_tolerance(add, start[b, :, :n] + add, bound, D, S * Hq // Hkv)).all(), (b, err.max())
+
+
 @pytest.mark.parametrize("S,at,Hq,Hkv,D,T", [(1, 100, 4, 1, 128, 400), (7, 0, 8, 1, 64, 500), (16, 30, 8, 2, 128, 512), (3, 5, 4, 4, 256, 2000),
                                              (20, 60, 6, 1, 128, 1500)])
 def test_prompt_weights_of_a_cache_with_room(S, at, Hq, Hkv, D, T):
