@@ -265,6 +265,54 @@ pub unsafe fn deltanet_decode_layer_gpu(mixed_qkv: *const c_void, conv_weight: *
                                              l2norm as c_int, stream))
 }
 
+/// One decode step and the softmax weights of its queries, added to `weights_in` (null: zeros) into `weights_out`:
+/// fp32 rows `[B, Hkv, weights_stride]`, one entry per cached token.  `k_new` and `v_new` null: attention only.
+///
+/// # Safety
+/// As above; `workspace` holds at least `hs_decode_weights_workspace_bytes(..)` bytes, 256-byte aligned.
+#[allow(clippy::too_many_arguments)]
+pub unsafe fn decode_step_weights_gpu(fp8: bool, q: *const c_void, k_new: *const c_void, v_new: *const c_void, src_dtype: c_int,
+                                      k_codes: *mut c_void, v_codes: *mut c_void, k_scales: *mut f32, v_scales: *mut f32,
+                                      layout: &hs_kv_layout, seq_lens: *const i32, out: *mut c_void, weights_in: *const f32,
+                                      weights_out: *mut f32, weights_stride: i64, workspace: *mut c_void,
+                                      workspace_bytes: usize, shape: AttnShape, max_seq_len: i32, softmax_scale: f32,
+                                      stream: hs_stream_t) -> Result<()> {
+    check(bindings::hs_decode_step_weights(fp8 as c_int, q, k_new, v_new, src_dtype, k_codes, v_codes, k_scales, v_scales,
+                                           layout, seq_lens, out, weights_in, weights_out, weights_stride, workspace,
+                                           workspace_bytes, shape.b, shape.hq, shape.hkv, shape.d, max_seq_len,
+                                           softmax_scale, stream))
+}
+
+/// The softmax weights of `s` queries per sequence over the cached keys, added to `weights_in` into `weights_out`.
+///
+/// # Safety
+/// As above; `workspace` holds at least `hs_attn_weights_workspace_bytes(..)` bytes, 256-byte aligned.
+#[allow(clippy::too_many_arguments)]
+pub unsafe fn attn_weights_gpu(fp8: bool, q: *const c_void, k_codes: *const c_void, k_scales: *const f32, layout: &hs_kv_layout,
+                               positions: *const i32, start_pos: i32, weights_in: *const f32, weights_out: *mut f32,
+                               weights_stride: i64, workspace: *mut c_void, workspace_bytes: usize, s: i32,
+                               shape: AttnShape, max_seq_len: i32, softmax_scale: f32, stream: hs_stream_t) -> Result<()> {
+    check(bindings::hs_attn_weights(fp8 as c_int, q, k_codes, k_scales, layout, positions, start_pos, weights_in, weights_out,
+                                    weights_stride, workspace, workspace_bytes, shape.b, s, shape.hq, shape.hkv, shape.d,
+                                    max_seq_len, softmax_scale, stream))
+}
+
+/// Cuts every sequence down to at most `budget` tokens per kv-head in place: the first `sinks`, the last `recent` and the
+/// heaviest of those between (`weights` null: the newest).
+///
+/// # Safety
+/// As above; `workspace` holds at least `hs_kv_evict_workspace_bytes(..)` bytes, 256-byte aligned.
+#[allow(clippy::too_many_arguments)]
+pub unsafe fn kv_evict_in_place_gpu(fp8: bool, k_codes: *mut c_void, v_codes: *mut c_void, k_scales: *mut f32, v_scales: *mut f32,
+                                    layout: &hs_kv_layout, seq_lens: *mut i32, weights: *mut f32, weights_stride: i64,
+                                    budget: i32, sinks: i32, recent: i32, workspace: *mut c_void, workspace_bytes: usize,
+                                    b: i32, hkv: i32, d: i32, max_seq_len: i32, stream: hs_stream_t) -> Result<()> {
+    check(bindings::hs_kv_evict(fp8 as c_int, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, weights, weights_stride,
+                                k_codes, v_codes, k_scales, v_scales, layout, seq_lens, weights, weights_stride,
+                                std::ptr::null_mut(), budget, sinks, recent, workspace, workspace_bytes, b, hkv, d,
+                                max_seq_len, stream))
+}
+
 /// Bytes of split-K workspace a decode call of this shape may need.
 pub fn decode_workspace_bytes(shape: AttnShape, max_seq_len: i32) -> usize {
     unsafe { bindings::hs_decode_attn_workspace_bytes(shape.b, shape.hq, shape.hkv, shape.d, max_seq_len) }
