@@ -12,6 +12,8 @@
 // short floats (e4m3fn) that fp16 and bf16 hold exactly, q is bf16.  Each kernel keeps its stationary side in registers
 // and converts only there or once per workgroup: columns as fp16 in the first (the streamed codes take one byte permute
 // and one subtraction per two), keys as bf16 in the second (the streamed q is used as it lies).
+// 4 x 4096 queries of 32 heads on their own keys (550 GFLOP in both products): 358 + 300 us under the profiler, 597 a call,
+// 920 TFLOP/s; the second kernel takes 219 without its LDS operand reads, which share the LDS with the tiles' copies.
 // The keys sit on the M axis, so a lane's four score registers are four keys of one column: row statistics stay in the
 // lane until the end of the walk, and so do the column sums.
 #include <algorithm>

@@ -6,6 +6,9 @@
 // order; it also moves their weights.  evict_move_kernel copies the listed code rows and scales, tiles of tokens in
 // parallel; evict_inplace_kernel does the same inside one buffer, where a tile may only be overwritten once it has been
 // read, with one workgroup per (sequence, kv-head, tensor) that walks its tiles in order.
+//
+// 64 x 8 rows of 8192 tokens cut to 1024 (D = 128; 300 MB of weights, kept rows read and written): 14 us of selection and 54
+// of copy at 5.3 TB/s.  8 rows of 32768 cut to 4096: 22 us, one workgroup's chain of passes over a row, and 5 of copy.
 #include <algorithm>
 
 #include "common.hpp"
