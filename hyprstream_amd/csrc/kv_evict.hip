@@ -10,6 +10,7 @@
 // 64 x 8 rows of 8192 tokens cut to 1024 (D = 128; 300 MB of weights, kept rows read and written): 14 us of selection and 54
 // of copy at 5.3 TB/s.  8 rows of 32768 cut to 4096: 22 us, one workgroup's chain of passes over a row, and 5 of copy.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -121,9 +122,10 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
 // does not count goes to a place of the lane's own), and sixteen wavefronts hide each other's latencies (with four per
 // row and 32 weights a thread: 25 us at 64 x 8 rows of 8192 tokens, 14 now).
 constexpr uint32_t kProtected = 0xffffffffu, kZeroKey = 0x80000000u;
+// Two workgroups share a CU where LDS lets them (64 registers: 14 us at 64 x 8 rows of 8192, 20 with 66).
 // MOVE: head_dim of the codes if the workgroup goes on to move its row's tokens itself, 0 if evict_move_kernel does.
 template <int TILE, int MOVE>
-__global__ __launch_bounds__(1024) void evict_select_kernel(EvictArgs a) {
+__global__ __launch_bounds__(1024, TILE == 8192 && MOVE == 0 ? 8 : 4) void evict_select_kernel(EvictArgs a) {
     constexpr int THREADS = 1024;
     constexpr uint32_t kCand = 1024;
     constexpr int kWaves = THREADS / 64, kGroup = 4 * THREADS, kGroups = TILE / kGroup, kCounts = kGroups * kWaves;
@@ -144,7 +146,7 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvictArgs a) {
         if (tid == 0) sm_first = s;
     } else {
         const int lo = a.sinks, hi = L - a.recent, K = a.budget - a.sinks - a.recent;
-        const int tiles = (L + TILE - 1) / TILE;
+        const int tiles = TILE == 8192 ? 1 : (L + TILE - 1) / TILE;  // (the small tile serves max_seq_len <= 8192)
         // keys of the tile that starts at `base`: every thread reads back only what it wrote.  Tokens behind the row
         // take key 0: the lowest one, and last among its equals.
         auto load = [&](int base) {
@@ -184,23 +186,40 @@ __global__ __launch_bounds__(1024) void evict_select_kernel(EvictArgs a) {
                 }
             } else {
                 uint32_t zeros = 0;  // tokens without any weight are many and would queue at one counter
+                auto count = [&](auto first_tag) {
+                    constexpr bool kFirst = decltype(first_tag)::value;
 #pragma unroll 1
-                for (int tile = 0; tile < tiles; ++tile) {
-                    if (tiles > 1) load(tile * TILE);
-                    const int left = L - tile * TILE - 4 * tid;  // tokens of the row from this thread's first one on
+                    for (int tile = 0; tile < tiles; ++tile) {
+                        if (tiles > 1) load(tile * TILE);
+                        const int left = L - tile * TILE - 4 * tid;  // tokens of the row from this thread's first one on
 #pragma unroll
-                    for (int i = 0; i < kGroups; ++i) {
-                        if (i * kGroup >= left) break;
-                        const u32x4 k = *(const u32x4 *)&sm_key[i * kGroup + 4 * tid];
+                        for (int i = 0; i < kGroups; ++i) {
+                            if (i * kGroup >= left) break;
+                            const u32x4 k = *(const u32x4 *)&sm_key[i * kGroup + 4 * tid];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const bool none = k[e] == kZeroKey && shift == 21;
-                            const bool counts = k[e] != kProtected && ((k[e] ^ prefix) & fixed) == 0u && !none && i * kGroup + e < left;
-                            zeros += none ? 1u : 0u;
-                            atomicAdd(&sm_hist[counts ? (k[e] >> shift) & mask : 2048u + lane], 1u);
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t own = 2048u + lane;
+                                if constexpr (kFirst) {
+                                    const bool none = k[e] == kZeroKey;
+                                    zeros += none ? 1u : 0u;
+                                    atomicAdd(&sm_hist[k[e] != kProtected && !none && i * kGroup + e < left ? k[e] >> 21 : own], 1u);
+                                } else {
+                                    // more than kCand keys share the first digit: often they are all equal, so lane 0 (whose
+                                    // tokens come first: it is there while any is) counts for every lane that shares its bin
+                                    // (8 rows of 32768, 1 % of them with a weight: 77 us without, 31 with; the first pass,
+                                    // where weights differ, loses 1 us of 26 to it)
+                                    const bool counts = k[e] != kProtected && ((k[e] ^ prefix) & fixed) == 0u && i * kGroup + e < left;
+                                    const uint32_t bin = counts ? (k[e] >> shift) & mask : own;
+                                    const bool led = bin == (uint32_t)__builtin_amdgcn_readfirstlane((int)bin);
+                                    const uint32_t many = (uint32_t)__popcll(__builtin_amdgcn_ballot_w64(led));
+                                    atomicAdd(&sm_hist[led && lane != 0 ? own : bin], lane == 0 ? many : 1u);
+                                }
+                            }
                         }
                     }
-                }
+                };
+                if (shift == 21) count(std::true_type{});
+                else count(std::false_type{});
                 if (shift == 21) {
                     zeros = (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(zeros), 63);
                     if (lane == 0 && zeros != 0) atomicAdd(&sm_hist[kZeroKey >> 21], zeros);

@@ -158,7 +158,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
     // skipped by that wavefront, steps that a bound cuts through take the masking path of the softmax.  The first a.sinks
     // tokens of the sequence stay visible: their steps (in the history, or in the call's own tokens where the history is
     // shorter than they are) come ahead of both walks.  (4 x 512 queries after 3584 tokens, window 1024, 4 sinks: 55 us, 630
-    // TFLOP/s of visible products; 1000 queries at head_dim 256 over a window of 2000: 93 us, on 64 workgroups.)
+    // TFLOP/s of visible products; 1000 queries at head_dim 256 over a window of 2000: 93 us, on 128 workgroups.)
     const int W = kWin && a.window > 0 ? a.window : (1 << 30);
     // in-call index of the first key column nb sees (negative: that many history tokens back)
     auto qlo = [&](int nb) { return min(qi[nb], S - 1) - W + 1; };

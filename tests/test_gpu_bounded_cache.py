@@ -143,7 +143,7 @@ LONG = [  # B, Hkv, D, T, lens, budget, sinks, recent, fp8, paged
 
 
 @pytest.mark.parametrize("case", LONG, ids=lambda c: "B%d-T%d-to%d" % (c[0], c[3], c[5]))
-@pytest.mark.parametrize("kind", ["smooth", "ties", "equal", None])
+@pytest.mark.parametrize("kind", ["smooth", "ties", "equal", "sparse", None])
 @pytest.mark.parametrize("where", ["out", "out-lens", "in"])
 def test_evict_long_rows(case, kind, where):
     B, Hkv, D, T, lens, budget, sinks, recent, fp8, paged = case
@@ -161,6 +161,23 @@ def test_evict_long_rows(case, kind, where):
         lo, wo = seq if where == "out-lens" else torch.zeros_like(seq), torch.full((B, Hkv, (budget + 3) // 4 * 4), 7.0, device=DEV)
     hb.kv_evict(c.tensors, c.layout, seq, wd, o.tensors, o.layout, lo, wo, ws, budget, sinks, recent, T, kept=kept, fp8=fp8)
     _check(c, o, w, lens, budget, sinks, recent, wo, lo, kept, src)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("src,dst", [(0, 64), (128, 0), (64, 128)])
+@pytest.mark.parametrize("budget", [50, 700])
+def test_evict_from_one_layout_to_another(fp8, src, dst, budget):
+    B, Hkv, D, T, lens = 3, 2, 128, 1000, (1000, 701, 33)
+    c = Cache(6250, B, Hkv, T, D, fp8=fp8, paged=src)
+    w = _weights(6251, B, Hkv, T, "smooth")
+    before = [c.dense(j).clone() for j in range(4)]
+    z = torch.zeros(B, budget, Hkv, D, dtype=torch.bfloat16, device=DEV)
+    o = Cache(6252, B, Hkv, budget, D, fp8=fp8, paged=dst, k=z, v=z)
+    seq, lo = torch.tensor(lens, dtype=torch.int32, device=DEV), torch.zeros(B, dtype=torch.int32, device=DEV)
+    kept, wo = torch.zeros(B, Hkv, budget, dtype=torch.int32, device=DEV), torch.full((B, Hkv, (budget + 3) // 4 * 4), 7.0, device=DEV)
+    hb.kv_evict(c.tensors, c.layout, seq, torch.from_numpy(w).to(DEV), o.tensors, o.layout, lo, wo, _space(hb.kv_evict_workspace_bytes(B, Hkv, budget, T)),
+                budget, 3, 20, T, kept=kept, fp8=fp8)
+    _check(c, o, w, lens, budget, 3, 20, wo, lo, kept, before)
 
 
 @pytest.mark.parametrize("fp8", [False, True])
@@ -246,8 +263,8 @@ def test_prompt_weights_of_uneven_queries(D, Hq, Hkv, S, at):
 
 
 @pytest.mark.parametrize("quant", [kc.INT8, kc.FP8])
-@pytest.mark.parametrize("window,sinks", [(0, 0), (96, 3)])
-def test_mirror_follows_the_calls(quant, window, sinks):
+@pytest.mark.parametrize("window,sinks,scratch", [(0, 0, 0), (96, 3, 0), (96, 3, 512)])
+def test_mirror_follows_the_calls(quant, window, sinks, scratch):
     """A session through LayerKVCache against the same calls on buffers of the test's own, bit for bit: prompt, steps,
     eviction, a truncation, a chunk behind it."""
     B, Hq, Hkv, D, cap, fp8 = 2, 8, 2, 128, 512, quant == kc.FP8
@@ -255,6 +272,8 @@ def test_mirror_follows_the_calls(quant, window, sinks):
     cache = kc.LayerKVCache(cap, quant)
     cache.set_window(window, sinks)
     cache.track_weights()
+    if scratch:
+        cache.enable_prompt_scratch(scratch)  # (a windowed prompt reads the codes and is not split: the same bits)
     c = Cache(6600, B, Hkv, cap, D, fp8=fp8)
     w = torch.zeros(B, Hkv, cap, device=DEV)
     n = 0

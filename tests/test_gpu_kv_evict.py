@@ -31,6 +31,8 @@ def _weights(stream, B, Hkv, T, kind):
         pick = r.integers(0, 9, w.shape)
         for i, x in enumerate([np.nan, np.inf, -np.inf, 0.0, -0.0, -1.5, 1e-42]):
             w[pick == i] = x
+    if kind == "sparse":  # most tokens never seen
+        w[r.random(w.shape) > 0.02] = 0
     if kind == "equal":
         w[:] = 0.25
     return w
@@ -56,7 +58,7 @@ def _check(c, c_out, w, lens, budget, sinks, recent, w_out, lens_out, kept, src)
 
 
 @pytest.mark.parametrize("case", CASES, ids=lambda c: "B%d-H%d-D%d-T%d-to%d-s%d-r%d-%s%s" % (c[:4] + c[5:8] + ("fp8" if c[8] else "int8", "-p%d" % c[9] if c[9] else "")))
-@pytest.mark.parametrize("kind", ["smooth", "ties", "odd", "equal", None])
+@pytest.mark.parametrize("kind", ["smooth", "ties", "odd", "equal", "sparse", None])
 @pytest.mark.parametrize("where", ["out", "in"])
 def test_evict(case, kind, where):
     B, Hkv, D, T, lens, budget, sinks, recent, fp8, paged = case
