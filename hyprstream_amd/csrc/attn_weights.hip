@@ -28,6 +28,10 @@ constexpr float kWLog2e = 1.4426950408889634f;
 constexpr int kWStep = 64;       // keys of a step of the first kernel
 constexpr int kCStepMax = 128;   // columns of a step of the second (64 at head_dim 256)
 constexpr int kWThreads = 256;   // both kernels
+// Statistics (key chunks x columns) up to which every workgroup of the narrow kernel joins them itself instead of a launch of
+// its own (us a call: 8 chunks x 64 columns 12.6 against 15.2, 512 x 8 27 against 33, 64 x 128 40.1 against 40.5, 256 x 128
+// 30.6 against 29.3).
+constexpr int kJoinMost = 8192;
 
 struct WeightsArgs {
     const uint16_t *q;   // [B, S, Hq, D] bf16
@@ -43,7 +47,7 @@ struct WeightsArgs {
     float *part_w;       // [segments, B, Hkv, part_stride] when the columns of a key block are split
     int64_t part_stride;
     int32_t start_pos, B, S, Hq, Hkv, G, cols, max_seq_len, window, sinks;
-    int32_t key_chunks, chunk_tokens, segments, lse_stride;
+    int32_t key_chunks, chunk_tokens, segments, lse_stride, joins;
     float scale_log2e;
 };
 
@@ -444,6 +448,33 @@ __global__ __launch_bounds__(kWThreads, 2) void weights_narrow_kernel(WeightsArg
         const int x = tid + kWThreads * i, c = x / CPR, cc = min(c, a.cols - 1), s = cc / a.G;
         copy16_to_lds(a.q + (((int64_t)b * a.S + s) * a.Hq + h * a.G + cc - s * a.G) * D + 8 * ((x % CPR) ^ (c & SWZ)), sm_q + 16 * (kWThreads * i + 64 * wave));
     }
+    // the columns' lse: from their key chunks where these are few, else weights_join_kernel has made them
+    constexpr int kCols = 16 * NB, kParts = kWThreads / kCols;
+    __shared__ float sm_jm[COLUMNS ? kParts : 1][kCols], sm_jl[COLUMNS ? kParts : 1][kCols];
+    const bool joins = COLUMNS && a.joins;
+    if (joins) {
+        const int c = tid % kCols;
+        const float *ml = a.part_ml + ((int64_t)unit * a.key_chunks * a.cols + min(c, a.cols - 1)) * 2;
+        float M = -3.0e38f, L = 0.0f;
+        for (int k0 = tid / kCols; k0 < a.key_chunks; k0 += 8 * kParts) {
+            float cm[8], cl[8], top = M;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int k = k0 + i * kParts;
+                const float2 x = *(const float2 *)(ml + (int64_t)min(k, a.key_chunks - 1) * a.cols * 2);
+                cm[i] = x.x;
+                cl[i] = k < a.key_chunks ? x.y : 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, cm[i]);
+            L *= __builtin_amdgcn_exp2f(M - top);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) L += cl[i] * __builtin_amdgcn_exp2f(cm[i] - top);
+            M = top;
+        }
+        sm_jm[tid / kCols][c] = M;
+        sm_jl[tid / kCols][c] = L;
+    }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     bf16x8 qop[NB][KG];
@@ -458,7 +489,17 @@ __global__ __launch_bounds__(kWThreads, 2) void weights_narrow_kernel(WeightsArg
             const u32x4 w = *(const u32x4 *)(sm_q + (c * CPR + ((KG * lq + j) ^ (c & SWZ))) * 16) & (uint32_t)~(pos[nb] >> 31);
             qop[nb][j] = pack_bf16x8(w[0], w[1], w[2], w[3]);
         }
-        m[nb] = COLUMNS ? a.lse[(int64_t)unit * a.lse_stride + 16 * nb + li] : 0.0f;
+        m[nb] = 0.0f;
+        if (COLUMNS && joins) {
+            float M = -3.0e38f, L = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) M = fmaxf(M, sm_jm[i][c]);
+#pragma unroll
+            for (int i = 0; i < kParts; ++i) L += sm_jl[i][c] * __builtin_amdgcn_exp2f(sm_jm[i][c] - M);
+            m[nb] = L == 0.0f || c >= a.cols ? INFINITY : M + __builtin_amdgcn_logf(L);
+        } else if (COLUMNS) {
+            m[nb] = a.lse[(int64_t)unit * a.lse_stride + c];
+        }
         l[nb] = 0.0f;
     }
     // the loads above end here: a wait for them inside the loop would be a wait for the keys of the steps ahead as well
@@ -890,7 +931,7 @@ template <int D, bool FP8, int NB>
 static void launch_narrow(const WeightsArgs &a, const WeightsPlan &p, hipStream_t st) {
     const int64_t units = (int64_t)a.B * a.Hkv;
     weights_narrow_kernel<D, FP8, NB, false><<<(unsigned)(units * p.key_chunks), kWThreads, 0, st>>>(a);
-    if (p.key_chunks > 1) weights_join_kernel<<<(unsigned)((units * p.lse_stride + 15) / 16), 256, 0, st>>>(a);
+    if (p.key_chunks > 1 && !a.joins) weights_join_kernel<<<(unsigned)((units * p.lse_stride + 15) / 16), 256, 0, st>>>(a);
     weights_narrow_kernel<D, FP8, NB, true><<<(unsigned)(units * p.key_chunks), kWThreads, 0, st>>>(a);
 }
 
@@ -965,6 +1006,7 @@ int hs_attn_weights(int fmt_fp8, const void *q, const void *k_codes, const float
     a.start_pos = start_pos; a.B = B; a.S = S; a.Hq = Hq; a.Hkv = Hkv; a.G = Hq / Hkv;
     a.cols = (int)p.cols; a.lse_stride = (int)p.lse_stride; a.max_seq_len = max_seq_len;
     a.window = layout->prefill_window; a.sinks = std::min(layout->attn_sinks, max_seq_len);
+    a.joins = p.narrow && p.key_chunks > 1 && p.key_chunks * p.cols <= kJoinMost;
     a.key_chunks = p.key_chunks; a.chunk_tokens = p.chunk_tokens; a.segments = p.segments;
     a.scale_log2e = softmax_scale * kWLog2e;
     hipStream_t st = (hipStream_t)stream;
