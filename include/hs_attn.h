@@ -415,7 +415,9 @@ HS_API int hs_attn_weights(int fmt_fp8, const void *q, const void *k_codes, cons
  *   *_out        where the tokens go: codes, int8 scales (fp8: the head scales are copied), by layout_out.  Either a cache
  *                of its own (any capacity >= budget, paged or not), or the source itself: the same buffers, tables and
  *                strides, which is done in place.  A layout_out that shares the source's buffers through other block
- *                tables must not share blocks with it.  int8 or fp8 as the source.
+ *                tables must not share blocks with it.  Sequences may share blocks of a source that is only read
+ *                (a common prefix); in place, and in layout_out, every block belongs to one sequence.  int8 or fp8 as
+ *                the source.  What lies behind the tokens that stay is left as it was.
  *   seq_lens_out device [B]: min(L, budget); may be seq_lens.
  *   weights_out  rows [B, Hkv, weights_out_stride] (alignment as above, stride >= budget): the weights of the kept tokens,
  *                then zeros up to min(weights_out_stride, max_seq_len); NULL = not wanted; may be `weights` if the stride is the same.

@@ -180,6 +180,27 @@ def test_evict_from_one_layout_to_another(fp8, src, dst, budget):
     _check(c, o, w, lens, budget, 3, 20, wo, lo, kept, before)
 
 
+def test_evict_of_sequences_that_share_blocks():
+    """Two sequences with the same blocks in front, as after a common prompt, into blocks of their own; what lies behind
+    the kept tokens there stays."""
+    B, Hkv, D, T, blk, budget = 2, 2, 128, 512, 64, 100
+    c = Cache(6260, B, Hkv, T, D, paged=blk)
+    for t in c.tables:
+        t[1, :4] = t[0, :4]
+    before = [c.dense(j).clone() for j in range(4)]
+    w = _weights(6261, B, Hkv, T, "smooth")
+    z = torch.zeros(B, 128, Hkv, D, dtype=torch.bfloat16, device=DEV)
+    o = Cache(6262, B, Hkv, 128, D, paged=blk, k=z, v=z)
+    for t in o.tensors:
+        t.fill_(9)
+    seq, lo = torch.tensor([512, 400], dtype=torch.int32, device=DEV), torch.zeros(B, dtype=torch.int32, device=DEV)
+    kept = torch.zeros(B, Hkv, budget, dtype=torch.int32, device=DEV)
+    hb.kv_evict(c.tensors, c.layout, seq, torch.from_numpy(w).to(DEV), o.tensors, o.layout, lo, None, _space(hb.kv_evict_workspace_bytes(B, Hkv, budget, T)),
+                budget, 4, 20, T, kept=kept)
+    _check(c, o, w, [512, 400], budget, 4, 20, None, lo, kept, before)
+    assert all((o.dense(j, 128)[:, :, budget:] == 9).all() for j in range(4))
+
+
 @pytest.mark.parametrize("fp8", [False, True])
 def test_strides_past_32_bits(fp8):
     """Sequences more than 2^31 bytes apart, weights rows more than 2^32: the same bits as over compact buffers."""
