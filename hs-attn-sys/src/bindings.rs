@@ -200,6 +200,7 @@ extern "C" {
     pub fn hs_paged_cache_prefill(c: *mut hs_paged_cache, q: *const c_void, new_keys: *const c_void, new_values: *const c_void, out: *mut c_void, seq_len: i32, num_q_heads: i32, start_pos: i64, softmax_scale: f32, stream: hs_stream_t) -> c_int;
     pub fn hs_paged_cache_clear(c: *mut hs_paged_cache);
     pub fn hs_paged_cache_truncate_to(c: *mut hs_paged_cache, pos: i64);
+    pub fn hs_paged_cache_evict(c: *mut hs_paged_cache, weights: *mut f32, weights_stride: i64, budget: i32, sinks: i32, recent: i32, stream: hs_stream_t) -> c_int;
     pub fn hs_paged_cache_seq_pos(c: *const hs_paged_cache) -> i64;
     pub fn hs_paged_cache_num_blocks(c: *const hs_paged_cache) -> i64;
     pub fn hs_paged_batch_decode_step(pool: *mut hs_pool, rows: *const *mut hs_paged_cache, n: i32, q: *const c_void, k_new: *const c_void, v_new: *const c_void, dtype: c_int, out: *mut c_void, num_q_heads: i32, softmax_scale: f32, stream: hs_stream_t) -> c_int;

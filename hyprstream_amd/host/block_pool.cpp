@@ -270,22 +270,49 @@ Status PagedLayerKVCache::get_dense(void *keys_out, void *values_out, int dtype,
     return from_abi(rc);
 }
 
+Status PagedLayerKVCache::grow_workspace(size_t bytes) {
+    if (bytes <= workspace_bytes_) return {};
+    if (workspace_) {
+        if (hipError_t e = hipDeviceSynchronize(); e != hipSuccess) return hip_err(e, "waiting before the workspace grows");
+        (void)hipFree(workspace_);
+    }
+    workspace_ = nullptr;
+    workspace_bytes_ = 0;
+    if (hipError_t e = hipMalloc(&workspace_, bytes); e != hipSuccess) {
+        workspace_ = nullptr;
+        return hip_err(e, "allocating the workspace");
+    }
+    workspace_bytes_ = bytes;
+    return {};
+}
+
+Status PagedLayerKVCache::evict(float *weights, int64_t weights_stride, int32_t budget, int32_t sinks, int32_t recent, hs_stream_t stream) {
+    if (seq_pos == 0) return err(HS_ERR_INVALID_ARGUMENT, "Cache is empty");
+    if (budget <= 0 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
+        return err(HS_ERR_INVALID_ARGUMENT, "need budget > 0 and 0 <= sinks + recent <= budget");
+    if ((size_t)budget >= seq_pos) return {};
+    if (Status s = sync_table(stream); !s.ok()) return s;
+    const int32_t heads = pool_->num_kv_heads(), dim = pool_->head_dim(), len = (int32_t)seq_pos;
+    if (Status s = grow_workspace(hs_kv_evict_workspace_bytes(1, heads, budget, len)); !s.ok()) return s;
+    if (hipError_t e = fill_i32(len_dev_, 1, len, (hipStream_t)stream); e != hipSuccess) return hip_err(e, "setting the length");
+    const int32_t stride = (int32_t)((max_seq_len + kBlockSize - 1) / kBlockSize);
+    const hs_kv_layout l = pool_->layout(table_dev_, table_dev_ + stride, stride);
+    float *ks = pool_->fp8() ? head_scales_dev_ : pool_->scales(), *vs = pool_->fp8() ? head_scales_dev_ + heads : ks;
+    const int rc = hs_kv_evict(pool_->fp8(), pool_->codes(), pool_->codes(), ks, vs, &l, len_dev_, weights, weights_stride,
+                               pool_->codes(), pool_->codes(), ks, vs, &l, len_dev_, weights, weights_stride, nullptr, budget, sinks,
+                               recent, workspace_, workspace_bytes_, 1, heads, dim, len, stream);
+    if (rc != HS_OK) return from_abi(rc);
+    truncate_to((size_t)budget);
+    return {};
+}
+
 Status PagedLayerKVCache::decode_attention(const void *q, void *out, int32_t hq, float scale, hs_stream_t stream) {
     if (seq_pos == 0) return err(HS_ERR_INVALID_ARGUMENT, "Cache is empty");
     if (Status s = sync_table(stream); !s.ok()) return s;
     const int32_t heads = pool_->num_kv_heads(), dim = pool_->head_dim();
-    const size_t need = hs_decode_attn_workspace_bytes(1, hq, heads, dim, (int32_t)max_seq_len);  // sized once
+    // (sized once)
+    if (Status s = grow_workspace(hs_decode_attn_workspace_bytes(1, hq, heads, dim, (int32_t)max_seq_len)); !s.ok()) return s;
     hipError_t e;
-    if (need > workspace_bytes_) {
-        if (workspace_) {
-            if ((e = hipDeviceSynchronize()) != hipSuccess) return hip_err(e, "waiting before the workspace grows");
-            (void)hipFree(workspace_);
-        }
-        workspace_ = nullptr;
-        workspace_bytes_ = 0;
-        if ((e = hipMalloc(&workspace_, need)) != hipSuccess) return hip_err(e, "allocating the workspace");
-        workspace_bytes_ = need;
-    }
     const int32_t len = (int32_t)seq_pos;
     if ((e = fill_i32(len_dev_, 1, len, (hipStream_t)stream)) != hipSuccess) return hip_err(e, "setting the length");
     const int32_t stride = (int32_t)((max_seq_len + kBlockSize - 1) / kBlockSize);

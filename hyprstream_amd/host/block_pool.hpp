@@ -104,6 +104,9 @@ class PagedLayerKVCache {
                    size_t start_pos, float softmax_scale, hs_stream_t stream = nullptr);
     void clear();
     void truncate_to(size_t pos);  // frees the blocks beyond the last needed one (kv_cache.rs:1725-1748)
+    // Keep `budget` tokens per kv-head (hs_kv_evict in place) and give the blocks behind them back to the pool.  weights:
+    // device [num_kv_heads, weights_stride], the kept tokens' entries moved with them; nullptr = the sinks and the newest.
+    Status evict(float *weights, int64_t weights_stride, int32_t budget, int32_t sinks, int32_t recent, hs_stream_t stream = nullptr);
     size_t num_blocks() const { return key_blocks_.size(); }
     const std::vector<BlockId> &key_blocks() const { return key_blocks_; }
     const std::vector<BlockId> &value_blocks() const { return value_blocks_; }
@@ -118,6 +121,7 @@ class PagedLayerKVCache {
 
   private:
     Status sync_table(hs_stream_t stream);
+    Status grow_workspace(size_t bytes);
     std::shared_ptr<BlockPool> pool_;
     CacheOwner owner_;
     std::vector<BlockId> key_blocks_, value_blocks_;

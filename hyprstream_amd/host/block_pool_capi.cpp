@@ -102,6 +102,11 @@ int hs_paged_cache_prefill(hs_paged_cache *c, const void *q, const void *new_key
 }
 void hs_paged_cache_clear(hs_paged_cache *c) { if (c) c->cache.clear(); }
 void hs_paged_cache_truncate_to(hs_paged_cache *c, int64_t pos) { if (c && pos >= 0) c->cache.truncate_to((size_t)pos); }
+int hs_paged_cache_evict(hs_paged_cache *c, float *weights, int64_t weights_stride, int32_t budget, int32_t sinks, int32_t recent,
+                         hs_stream_t stream) {
+    if (!c) return HS_ERR_INVALID_ARGUMENT;
+    return c->done(c->cache.evict(weights, weights_stride, budget, sinks, recent, stream));
+}
 int64_t hs_paged_cache_seq_pos(const hs_paged_cache *c) { return c ? (int64_t)c->cache.seq_pos : 0; }
 int64_t hs_paged_cache_num_blocks(const hs_paged_cache *c) { return c ? (int64_t)c->cache.num_blocks() : 0; }
 

@@ -21,7 +21,7 @@ EXPORTS = [
     "hs_pool_create", "hs_pool_create_format", "hs_pool_quant_type", "hs_pool_destroy", "hs_pool_last_error", "hs_pool_allocate", "hs_pool_free", "hs_pool_owner_of",
     "hs_pool_used_blocks", "hs_pool_free_block_count", "hs_pool_total_blocks", "hs_pool_used_memory",
     "hs_paged_cache_create", "hs_paged_cache_destroy", "hs_paged_cache_last_error", "hs_paged_cache_update",
-    "hs_paged_cache_get_dense", "hs_paged_cache_decode_attention", "hs_paged_cache_clear", "hs_paged_cache_truncate_to",
+    "hs_paged_cache_get_dense", "hs_paged_cache_decode_attention", "hs_paged_cache_clear", "hs_paged_cache_truncate_to", "hs_paged_cache_evict",
     "hs_paged_cache_seq_pos", "hs_paged_cache_num_blocks", "hs_paged_batch_decode_step",
     "hs_compat_create", "hs_compat_destroy", "hs_compat_set_uint", "hs_compat_set_opt_uint", "hs_compat_set_str",
     "hs_compat_add_layer_type", "hs_compat_set_rope_scaling", "hs_compat_set_kv_quant",
@@ -340,6 +340,13 @@ class PagedLayerKVCache(_Handle):
 
     def truncate_to(self, pos):
         lib().hs_paged_cache_truncate_to(self._h, ctypes.c_int64(pos))
+
+    def evict(self, budget, sinks=0, recent=0, weights=None):
+        """Keep `budget` tokens per kv-head and give the blocks behind them back; weights: fp32 [Hkv, stride], moved along."""
+        assert weights is None or (weights.is_contiguous() and weights.shape[0] == self.pool.num_kv_heads and str(weights.dtype) == "torch.float32")
+        stride = 0 if weights is None else weights.shape[1]
+        self._check(lib().hs_paged_cache_evict(self._h, hb._ptr(weights), ctypes.c_int64(stride), ctypes.c_int32(budget),
+                                               ctypes.c_int32(sinks), ctypes.c_int32(recent), hb._stream()))
 
 
 def paged_batch_decode_step(pool, rows, q, k_new, v_new, softmax_scale):

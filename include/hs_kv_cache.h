@@ -178,6 +178,12 @@ HS_API int hs_paged_cache_prefill(hs_paged_cache *c, const void *q, const void *
                                   hs_stream_t stream);
 HS_API void hs_paged_cache_clear(hs_paged_cache *c);
 HS_API void hs_paged_cache_truncate_to(hs_paged_cache *c, int64_t pos);
+/* Keeps `budget` tokens per kv-head in place, as hs_cache_evict does, and gives the blocks behind them back to the pool.
+ * weights: device fp32 [num_kv_heads, weights_stride], one entry per cached token (hs_decode_step_weights and
+ * hs_attn_weights on the cache's block table fill such rows), moved with the tokens that stay; NULL = the first `sinks` and
+ * the newest.  As after hs_paged_cache_truncate_to, work queued on other streams must not still read the blocks. */
+HS_API int hs_paged_cache_evict(hs_paged_cache *c, float *weights, int64_t weights_stride, int32_t budget, int32_t sinks,
+                                int32_t recent, hs_stream_t stream);
 HS_API int64_t hs_paged_cache_seq_pos(const hs_paged_cache *c);
 HS_API int64_t hs_paged_cache_num_blocks(const hs_paged_cache *c); /* K blocks held (= V blocks held) */
 

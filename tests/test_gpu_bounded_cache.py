@@ -402,6 +402,49 @@ def test_mirror_bounds_an_endless_session():
             assert (np.abs(f64(out[0]) - ref[0]) <= decode_tolerance(ref, mag, bound)[0]).all()
 
 
+@pytest.mark.parametrize("quant", [kc.INT8, kc.FP8])
+@pytest.mark.parametrize("counted", [False, True])
+def test_paged_mirror_gives_blocks_back(quant, counted):
+    """Eviction through a paged cache: the tokens that stay are the right ones, their blocks too, the others are free, and
+    another cache of the pool keeps what it holds."""
+    H, D, n = 2, 64, 1100
+    pool = kc.BlockPool(24, H, D, quant)
+    one, two = kc.PagedLayerKVCache(2048, pool, "one"), kc.PagedLayerKVCache(2048, pool, "two")
+    k, v = bf16_randn(6750, 1, n, H, D), bf16_randn(6751, 1, n, H, D)
+    two.update(k[:, :300], v[:, :300], 0)
+    one.update(k, v, 0)
+    other, before = [t.clone() for t in two.get(torch.float32)], [t.clone() for t in one.get(torch.float32)]
+    w = _weights(6752, 1, H, n, "smooth")[0] if counted else None
+    wd = torch.from_numpy(w).to(DEV) if counted else None
+    assert one.num_blocks == 5
+    one.evict(300, 4, 100, weights=wd)
+    assert one.seq_pos == 300 and one.num_blocks == 2 and pool.used_blocks() == 8
+    want = [keep(None if w is None else w[h], n, 300, 4, 100) for h in range(H)]
+    after = one.get(torch.float32)
+    for h in range(H):
+        idx = torch.from_numpy(want[h]).to(DEV)
+        assert all(torch.equal(a[0, :, h], b[0, idx, h]) for a, b in zip(after, before))
+        assert w is None or np.array_equal(wd[h, :300].cpu().numpy(), w[h][want[h]])
+    assert all(torch.equal(a, b) for a, b in zip(two.get(torch.float32), other))
+    q = bf16_randn(6753, 1, 4, D)
+    out = one.decode_attention(q, D ** -0.5)
+    K, V = (f64(t)[0] for t in one.get(torch.float32))
+    ref, _, mag, bound = attention(f64(q), K, V, [299], 0, 0, D ** -0.5)
+    assert (np.abs(f64(out) - ref) <= decode_tolerance(ref, mag, bound)).all()
+    one.update(k[:, :200], v[:, :200], 300)  # into blocks taken anew
+    assert one.seq_pos == 500 and all(torch.equal(a[:, :300], b) for a, b in zip(one.get(torch.float32), after))
+    one.evict(600)
+    assert one.seq_pos == 500
+    for bad in ((0, 0, 0), (8, 5, 4), (8, -1, 0)):
+        with pytest.raises(kc.CacheError, match="sinks"):
+            one.evict(*bad)
+    with pytest.raises(kc.CacheError, match="weights_stride"):
+        one.evict(8, weights=torch.zeros(H, 400, device=DEV))
+    one.clear()
+    with pytest.raises(kc.CacheError, match="empty"):
+        one.evict(8)
+
+
 def test_mirror_refusals():
     cache = kc.LayerKVCache(64)
     with pytest.raises(kc.CacheError, match="empty"):
