@@ -89,16 +89,12 @@ __device__ __forceinline__ bf16x8 codes_to_bf16(uint32_t w0, uint32_t w1) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const uint32_t w = i < 2 ? w0 : w1;
-        float lo, hi;
         if constexpr (FP8) {
-            const auto f = (i & 1) ? __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true) : __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
-            lo = f[0];
-            hi = f[1];
+            o[i] = __builtin_bit_cast(uint32_t, (i & 1) ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
         } else {
-            lo = (float)(int8_t)(w >> (16 * (i & 1)));
-            hi = (float)(int8_t)(w >> (16 * (i & 1) + 8));
+            const float lo = (float)(int8_t)(w >> (16 * (i & 1))), hi = (float)(int8_t)(w >> (16 * (i & 1) + 8));
+            o[i] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);  // the upper halves
         }
-        o[i] = __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);  // the upper halves
     }
     return pack_bf16x8(o[0], o[1], o[2], o[3]);
 }
