@@ -250,7 +250,7 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
     if (!kShadow && H > 0 && (!kSplit || h_lo < h_hi)) {
         // The history operands are fp16(code * scale), and fp16 spans 2^-14 .. 65504 only.  Each (sequence, kv-head)
         // therefore gets a power-of-two reference for K and one for V, taken from the largest scale among its first
-        // cached tokens (int8; up to 64 of them, inside one block) or from its head scale (fp8): operands are
+        // cached tokens (int8; up to 64 of them, inside one block; with a window the first visible ones) or from its head scale (fp8): operands are
         // fp16(code * scale * 2^-E), with that reference scale landing in [1/8, 1/4).  K's 2^E goes into the Q
         // operands, V's into the accumulators when the history ends -- both exact.  What matters is then a scale's
         // size RELATIVE to the head's own: rows up to 2^11 above the reference and down to 2^-11 below it keep full
@@ -261,6 +261,22 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
             if (FP8) {
                 rk = a.ks[(int64_t)b * a.Hkv + kvh];
                 rv = a.vs[(int64_t)b * a.Hkv + kvh];
+            } else if (kWin) {
+                // Only tokens that some query of the workgroup sees: the first of the window and of the sinks (what the
+                // window hides may hold anything; so no bit of the output depends on it).
+                auto first_scales = [&](const KvAddr &ad, const float *scales, int t0, int t1) {  // lane's of [t0, t0 + 64) below t1
+                    int64_t unit;
+                    int slot;
+                    float s = 0.0f;
+                    if (lane < t1 - t0 && resolve(ad, b, t0 + lane, unit, slot))
+                        s = scales[unit * ad.scale_stride_seq + (int64_t)kvh * ad.scale_stride_head + slot];
+                    return s < 3.0e38f ? s : 0.0f;
+                };
+                const int w0 = max(H + wg_lo, 0), sink_end = min(a.sinks, min(w0, H));
+                rk = fmaxf(first_scales(a.ka, a.ks, w0, H), first_scales(a.ka, a.ks, 0, sink_end));
+                rv = fmaxf(first_scales(a.va, a.vs, w0, H), first_scales(a.va, a.vs, 0, sink_end));
+                rk = wave_max(rk);
+                rv = wave_max(rv);
             } else {
                 int64_t unit;
                 int slot;
@@ -270,10 +286,6 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 16 ? 4 : 2) void prefill_att
                 resolve(a.va, b, 0, unit, slot);
                 n = min(min(H, 64), a.va.capacity_tokens - slot);
                 rv = a.vs[unit * a.va.scale_stride_seq + (int64_t)kvh * a.va.scale_stride_head + slot + min(lane, n - 1)];
-                if (kWin) {  // (a token the window hides may hold anything)
-                    rk = rk < 3.0e38f ? rk : 0.0f;
-                    rv = rv < 3.0e38f ? rv : 0.0f;
-                }
                 rk = wave_max(rk);
                 rv = wave_max(rv);
             }

@@ -114,8 +114,8 @@ typedef struct hs_kv_layout {
     int32_t attn_sinks;         /* with a window (prefill_window, decode_window), optional: the first attn_sinks tokens of
                                    a sequence stay visible whatever the window has left behind.  0 = none; without a
                                    window it changes nothing.  The scales of cached tokens that a query tile (prefill:
-                                   up to 256 (query, head) columns) does not see may be no numbers; a call's own K and V
-                                   rows have to be. */
+                                   up to 256 (query, head) columns) does not see may hold anything; a call's own K and V
+                                   rows have to be numbers. */
                                 /* prefill_split_workspace, prefill_key_splits: prefill only, optional: device scratch that lets a call whose query tiles are too few
                                    to occupy the GPU (a chunk of ONE sequence: 64 tiles on 256 compute units) cut the
                                    keys of every tile into runs for several workgroups, the last of which to finish

@@ -1,0 +1,48 @@
+"""Corners of a bounded cache: what the window hides, layouts and buffers that outlive a call, calls that are refused."""
+
+import pytest
+import torch
+
+from hyprstream_amd import bindings as hb
+from bounded_util import Cache, DEV, bf16_randn
+
+pytestmark = pytest.mark.gpu
+
+
+def _space(n):
+    return torch.full((max(256, n),), 0xFF, dtype=torch.uint8, device=DEV)
+
+
+# ---- windowed prefill: the power of two its operands are relative to
+HIDDEN = [  # B, S, T, Hq, Hkv, D, window, sinks, paged
+    (2, 40, 500, 8, 2, 64, 101, 5, 0),
+    (2, 40, 500, 8, 2, 128, 101, 5, 0),
+    (2, 40, 500, 8, 2, 256, 101, 5, 0),
+    (1, 40, 500, 8, 2, 128, 101, 0, 0),     # all of the first 64 tokens are hidden
+    (1, 300, 700, 8, 2, 64, 70, 0, 64),     # several query tiles, the window starts anywhere in a block
+    (1, 200, 333, 8, 2, 128, 129, 70, 64),  # more sinks than the reference looks at
+    (1, 1, 449, 8, 2, 256, 2, 0, 64),       # one visible history token, the first of its block
+]
+
+
+@pytest.mark.parametrize("case", HIDDEN, ids=lambda c: "B%d-S%d-T%d-%d/%d-D%d-w%d-s%d-p%d" % c)
+def test_finite_scales_of_hidden_tokens_do_not_matter(case):
+    """Prefill's history operands are fp16 relative to a power of two chosen from scales: of tokens some query of the tile
+    sees, so whatever the hidden ones hold, every bit of the output stays."""
+    B, S, T, Hq, Hkv, D, window, sinks, paged = case
+    q, kn, vn = bf16_randn(7000, B, S, Hq, D), bf16_randn(7001, B, S, Hkv, D), bf16_randn(7002, B, S, Hkv, D)
+    outs = []
+    for fill in (None, 1e30, 1e-30, 0.0, 2.0 ** 13, 2.0 ** -13, float("nan"), float("inf")):
+        c = Cache(7003, B, Hkv, T, D, paged=paged)
+        if fill is not None:  # tokens [sinks, T - window]: hidden from the query at T and from every later one
+            relative = 2.0 ** -13 <= fill <= 2.0 ** 13
+            for j in (2, 3):
+                s = c.tensors[j]
+                for b in range(B):
+                    for t in range(sinks, T - window + 1):
+                        at = (int(c.tables[j & 1][b, t // paged]), slice(None), t % paged) if paged else (b, slice(None), t)
+                        s[at] = s[at] * fill if relative else fill
+        out = torch.full((B, S, Hq, D), float("nan"), dtype=torch.bfloat16, device=DEV)
+        hb.prefill_attn(q, kn, vn, *c.tensors, c.layout, T, out, D ** -0.5, quantize_on_write=False, window=window, sinks=sinks)
+        outs.append(out)
+        assert torch.equal(out, outs[0]), (fill, (out.float() - outs[0].float()).abs().max().item())
