@@ -68,7 +68,7 @@ Status LayerKVCache::ensure_storage(int32_t batch, int32_t heads, int32_t dim) {
     layout_.scale_stride_head = (int64_t)cap_s;
     layout_.scale_stride_seq = (int64_t)cap_s * heads;
     layout_.capacity_tokens = (int32_t)cap;
-    layout_.decode_window = window_;
+    layout_.prefill_window = layout_.decode_window = window_;
     layout_.attn_sinks = sinks_;
     const size_t code_bytes = (size_t)batch * heads * cap * dim;
     const size_t scale_bytes = quant_type_ == KVQuantType::Fp8 ? (size_t)batch * heads * 4 : (size_t)batch * heads * cap_s * 4;
@@ -106,7 +106,7 @@ Status LayerKVCache::ensure_scratch(int32_t hq, int32_t batch, hs_stream_t strea
 
 Status LayerKVCache::set_window(int32_t window, int32_t sinks) {
     if (window < 0 || sinks < 0) return err(HS_ERR_INVALID_ARGUMENT, "negative window or sinks");
-    layout_.decode_window = window_ = window;
+    layout_.prefill_window = layout_.decode_window = window_ = window;
     layout_.attn_sinks = sinks_ = sinks;
     return {};
 }
@@ -316,7 +316,6 @@ Status LayerKVCache::prefill(const void *q, const void *new_keys, const void *ne
     if (Status s = clean_weights(start_pos, stream); !s.ok()) return s;
     int rc;
     hs_kv_layout lay = layout_;
-    lay.prefill_window = window_;
     bool with_copy = false;
     if (prompt_tokens_ > 0) {
         // key-split workspace: sized for the longest chunk seen (grows like the decode workspace)

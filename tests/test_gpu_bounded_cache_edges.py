@@ -1,9 +1,11 @@
 """Corners of a bounded cache: what the window hides, layouts and buffers that outlive a call, calls that are refused."""
+import ctypes
 
 import pytest
 import torch
 
 from hyprstream_amd import bindings as hb
+from hyprstream_amd import kv_cache as kc
 from bounded_util import Cache, DEV, bf16_randn
 
 pytestmark = pytest.mark.gpu
@@ -46,3 +48,41 @@ def test_finite_scales_of_hidden_tokens_do_not_matter(case):
         hb.prefill_attn(q, kn, vn, *c.tensors, c.layout, T, out, D ** -0.5, quantize_on_write=False, window=window, sinks=sinks)
         outs.append(out)
         assert torch.equal(out, outs[0]), (fill, (out.float() - outs[0].float()).abs().max().item())
+
+
+# ---- the mirror: its view, its buffers, calls it refuses
+def _view(cache):
+    """(k_codes, v_codes, k_scales, v_scales) as addresses, and the layout, of a LayerKVCache."""
+    lay, p = hb.KvLayout(), [ctypes.c_void_p() for _ in range(4)]
+    cache._check(kc.lib().hs_cache_get_view(cache._h, *[ctypes.byref(x) for x in p], ctypes.byref(lay), None, None, None))
+    return p, lay
+
+
+@pytest.mark.parametrize("early", [False, True])
+def test_view_carries_the_whole_window(early):
+    """The layout that a windowed cache gives out windows the calls it is handed to: prefill and the prompt's weights as
+    much as decode."""
+    B, S, H, Hq, Hkv, D, window, sinks = 2, 60, 200, 8, 2, 128, 50, 3
+    cache = kc.LayerKVCache(H + S)
+    if early:
+        cache.set_window(window, sinks)
+    k, v = bf16_randn(7100, B, H, Hkv, D), bf16_randn(7101, B, H, Hkv, D)
+    cache.update(k, v, 0)
+    if not early:
+        cache.set_window(window, sinks)
+    cache.track_weights()
+    q, kn, vn = bf16_randn(7102, B, S, Hq, D), bf16_randn(7103, B, S, Hkv, D), bf16_randn(7104, B, S, Hkv, D)
+    want = cache.prefill(q, kn, vn, H, D ** -0.5)
+    p, lay = _view(cache)
+    assert (lay.prefill_window, lay.decode_window, lay.attn_sinks) == (window, window, sinks)
+    got, T = torch.empty_like(want), H + S
+    L = hb.lib()
+    hb.check(L.hs_prefill_attn_int8(q.data_ptr(), kn.data_ptr(), vn.data_ptr(), *p, ctypes.addressof(lay), H, got.data_ptr(), B, S, Hq, Hkv,
+                                    D, D ** -0.5, 0, hb._stream()))
+    w, ws = torch.zeros(B, Hkv, T, device=DEV), _space(hb.attn_weights_workspace_bytes(B, S, Hq, Hkv, D, T))
+    hb.check(L.hs_attn_weights(0, q.data_ptr(), p[0], p[2], ctypes.addressof(lay), None, H, None, w.data_ptr(), T, ws.data_ptr(), ws.numel(),
+                               B, S, Hq, Hkv, D, T, D ** -0.5, hb._stream()))
+    assert torch.equal(got, want) and torch.equal(w, cache.weights())
+    cache.set_window(0)
+    _, lay = _view(cache)
+    assert (lay.prefill_window, lay.decode_window, lay.attn_sinks) == (0, 0, 0)
