@@ -923,6 +923,29 @@ static WeightsPlan plan_weights(int B, int S, int Hq, int Hkv, int D, int max_se
     return p;
 }
 
+// Most floats that a call with THESE sizes, or with fewer queries or a smaller max_seq_len, takes: a caller sizes its
+// workspace once, for its longest chunk and the capacity of its cache.  plan_weights's own sum falls and rises with either
+// (chunks are rounded, and the fewer there are of one thing the more another is split), hence a bound of each part.
+static size_t most_floats(int B, int S, int Hq, int Hkv, int D, int max_seq_len) {
+    const int64_t units = (int64_t)B * Hkv, cols = (int64_t)S * (Hq / Hkv), n = max_seq_len;
+    const int64_t most = D == 256 ? 64 : 128, few = std::min(cols, most);  // columns of a narrow call
+    const int64_t wg_cols = 2 * most, wg_keys = kWThreads / 4 * (D == 256 ? 2 : 4);
+    int64_t lse = few <= 32 ? 32 : few <= 64 ? 64 : 128;
+    // narrow: chunks of at least 128 keys, `want` of them at most unless they reach 4096 keys
+    const int64_t want = std::max<int64_t>(1, 512 / std::max<int64_t>(1, units));
+    const int64_t chunks = std::min((n + 127) / 128, std::max(want, (n + 4095) / 4096));
+    int64_t ml = chunks > 1 ? units * chunks * few * 2 : 0, w = 0;
+    if (cols > most) {
+        lse = std::max(lse, (cols + 127) / 128 * 128);
+        // wide: chunks of at least 512 keys, and only while units x column blocks x chunks stay within 1024
+        if (n > 512) ml = std::max(ml, 2 * std::min(units * ((n + 511) / 512) * cols, 1024 * wg_cols));
+        // shares of the columns: at most 16, no more than there are steps, and only up to 1024 + items
+        const int64_t items = units * ((n + wg_keys - 1) / wg_keys), steps = (cols + kCStepMax - 1) / kCStepMax;
+        if (steps > 1) w = wg_keys * std::min(std::min<int64_t>(steps, 16) * items, 1023 + std::min<int64_t>(items, 1023));
+    }
+    return (size_t)(units * lse + ml + w);
+}
+
 template <int D, bool FP8, int NB>
 static void launch_narrow(const WeightsArgs &a, const WeightsPlan &p, hipStream_t st) {
     const int64_t units = (int64_t)a.B * a.Hkv;
@@ -951,8 +974,7 @@ extern "C" {
 
 size_t hs_attn_weights_workspace_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_seq_len) {
     if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || (D != 64 && D != 128 && D != 256) || max_seq_len <= 0) return 0;
-    const hs::WeightsPlan p = hs::plan_weights(B, S, Hq, Hkv, D, max_seq_len);
-    return ((p.ml_floats + p.lse_floats + p.w_floats) * sizeof(float) + 255) / 256 * 256;
+    return (hs::most_floats(B, S, Hq, Hkv, D, max_seq_len) * sizeof(float) + 255) / 256 * 256;
 }
 
 int hs_attn_weights(int fmt_fp8, const void *q, const void *k_codes, const float *k_scales, const hs_kv_layout *layout,
@@ -984,7 +1006,7 @@ int hs_attn_weights(int fmt_fp8, const void *q, const void *k_codes, const float
     const int64_t units = (int64_t)B * Hkv;
     if (p.cols > INT32_MAX / 2 || units > 65535 || units * p.key_chunks * p.col_blocks > INT32_MAX || units * p.segments * p.key_blocks > INT32_MAX)
         return fail(HS_ERR_INVALID_ARGUMENT, "too large for one call (B=%d S=%d Hq=%d Hkv=%d)", B, S, Hq, Hkv);
-    const size_t need = hs_attn_weights_workspace_bytes(B, S, Hq, Hkv, D, max_seq_len);
+    const size_t need = (p.ml_floats + p.lse_floats + p.w_floats) * sizeof(float);  // (of this call; the size function's answer covers smaller ones)
     if (!workspace || workspace_bytes < need)
         return fail(HS_ERR_WORKSPACE, "workspace of %zu bytes given, %zu needed", workspace_bytes, need);
     if (((uintptr_t)workspace & 255) != 0) return fail(HS_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");

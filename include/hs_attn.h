@@ -399,7 +399,8 @@ HS_API int hs_decode_step_weights(int fmt_fp8, const void *q, const void *k_new,
  * below min(max_seq_len, last query's position + 1).  Keys are the DEQUANTIZED ones: hs_prefill_attn_* attends its own call's tokens
  * in bf16, so its weights differ by the quantization of those keys.  D is 64, 128 or 256; a paged layout needs
  * capacity_tokens to be a multiple of 64, as for prefill.  Workspace:
- * hs_attn_weights_workspace_bytes(...) bytes, 256-byte aligned. */
+ * hs_attn_weights_workspace_bytes(...) bytes, 256-byte aligned; they also serve every call with a smaller S or max_seq_len,
+ * so a cache's workspace is sized once, for its capacity and the longest chunk. */
 HS_API size_t hs_attn_weights_workspace_bytes(int32_t B, int32_t S, int32_t Hq, int32_t Hkv, int32_t D, int32_t max_seq_len);
 HS_API int hs_attn_weights(int fmt_fp8, const void *q, const void *k_codes, const float *k_scales,
                                const hs_kv_layout *layout, const int32_t *positions, int32_t start_pos,
