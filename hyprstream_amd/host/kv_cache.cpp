@@ -38,6 +38,8 @@ void LayerKVCache::release() {
     drop_prompt_scratch();
     for (void *p : {k_codes_, v_codes_, (void *)k_scales_, (void *)v_scales_, (void *)seq_lens_dev_, workspace_, (void *)weights_, bound_ws_})
         if (p) (void)hipFree(p);
+    for (void *p : outgrown_) (void)hipFree(p);
+    outgrown_.clear();
     weights_ = nullptr;
     bound_ws_ = nullptr;
     weights_stride_ = 0;
@@ -86,10 +88,9 @@ Status LayerKVCache::ensure_storage(int32_t batch, int32_t heads, int32_t dim) {
 }
 
 // The split-K workspace is sized ONCE for max_seq_len (it only ever grows if a later call brings more query heads),
-// so steady-state steps neither allocate nor free.  The sequence lengths reach the device through a fill launch on
-// the caller's stream, ordered with the attention launch that reads them.
-Status LayerKVCache::ensure_scratch(int32_t hq, int32_t batch, hs_stream_t stream) {
-    const size_t bytes = hs_decode_attn_workspace_bytes(batch, hq, heads_, dim_, (int32_t)max_seq_len);
+// so steady-state steps neither allocate nor free.
+Status LayerKVCache::ensure_scratch(int32_t hq) {
+    const size_t bytes = hs_decode_attn_workspace_bytes(batch_, hq, heads_, dim_, (int32_t)max_seq_len);
     if (bytes > workspace_bytes_) {
         if (workspace_) {
             // an earlier step on some stream may still use the old buffer
@@ -101,7 +102,12 @@ Status LayerKVCache::ensure_scratch(int32_t hq, int32_t batch, hs_stream_t strea
         if (hipError_t e = hipMalloc(&workspace_, bytes); e != hipSuccess) return hip_err(e, "allocating the workspace");
         workspace_bytes_ = bytes;
     }
-    return hip_err(fill_i32(seq_lens_dev_, batch, (int32_t)seq_pos, (hipStream_t)stream), "setting the sequence lengths");
+    return {};
+}
+
+// The sequence lengths reach the device through a fill launch on the caller's stream, ordered with the launch that reads them.
+Status LayerKVCache::set_lengths(hs_stream_t stream) {
+    return hip_err(fill_i32(seq_lens_dev_, batch_, (int32_t)seq_pos, (hipStream_t)stream), "setting the sequence lengths");
 }
 
 Status LayerKVCache::set_window(int32_t window, int32_t sinks) {
@@ -124,8 +130,12 @@ Status LayerKVCache::track_weights(bool on) {
     return {};
 }
 
-// The rows (when tracking) and a workspace of at least `bytes`, which only ever grows.
-Status LayerKVCache::ensure_weights(size_t bytes, hs_stream_t stream) {
+// The rows (when tracking) and a workspace for evictions, for counting steps of hq query heads and for counting prompts of
+// up to seq_len tokens (hq, seq_len 0: none).  Sizes are for max_seq_len tokens, so a session allocates at its first counting
+// call and again only for a longer chunk or more heads.  An outgrown workspace is kept until the storage goes: queued work
+// and captured graphs may still use it.  (It at least doubles, so those kept are no more than the one in use.)
+Status LayerKVCache::ensure_weights(int32_t hq, int32_t seq_len, hs_stream_t stream) {
+    const int32_t cap = (int32_t)max_seq_len;
     if (track_ && !weights_) {
         weights_stride_ = (int64_t)((max_seq_len + 3) / 4 * 4);
         const size_t n = (size_t)batch_ * heads_ * weights_stride_;
@@ -138,17 +148,16 @@ Status LayerKVCache::ensure_weights(size_t bytes, hs_stream_t stream) {
             return hip_err(e, "clearing the weights");
         weights_dirty_ = 0;
     }
+    size_t bytes = hs_kv_evict_workspace_bytes(batch_, heads_, cap, cap);
+    if (hq % heads_ != 0) hq = 0;  // (will be refused)
+    if (hq > 0) bytes = std::max(bytes, hs_decode_weights_workspace_bytes(batch_, hq, heads_, dim_, cap));
+    if (hq > 0 && seq_len > 0) bytes = std::max(bytes, hs_attn_weights_workspace_bytes(batch_, seq_len, hq, heads_, dim_, cap));
     if (bytes > bound_ws_bytes_) {
-        if (bound_ws_) {
-            if (hipError_t e = hipDeviceSynchronize(); e != hipSuccess) return hip_err(e, "waiting before the workspace grows");
-            (void)hipFree(bound_ws_);
-        }
-        bound_ws_ = nullptr;
-        bound_ws_bytes_ = 0;
-        if (hipError_t e = hipMalloc(&bound_ws_, bytes); e != hipSuccess) {
-            bound_ws_ = nullptr;
-            return hip_err(e, "allocating the workspace");
-        }
+        bytes = std::max(bytes, 2 * bound_ws_bytes_);
+        void *p = nullptr;
+        if (hipError_t e = hipMalloc(&p, bytes); e != hipSuccess) return hip_err(e, "allocating the workspace");
+        if (bound_ws_) outgrown_.push_back(bound_ws_);
+        bound_ws_ = p;
         bound_ws_bytes_ = bytes;
     }
     return {};
@@ -175,9 +184,8 @@ Status LayerKVCache::evict(int32_t budget, int32_t sinks, int32_t recent, hs_str
     if (budget <= 0 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
         return err(HS_ERR_INVALID_ARGUMENT, "need budget > 0 and 0 <= sinks + recent <= budget");
     if ((size_t)budget >= seq_pos) return {};
-    if (Status s = ensure_weights(hs_kv_evict_workspace_bytes(batch_, heads_, budget, (int32_t)seq_pos), stream); !s.ok()) return s;
-    if (hipError_t e = fill_i32(seq_lens_dev_, batch_, (int32_t)seq_pos, (hipStream_t)stream); e != hipSuccess)
-        return hip_err(e, "setting the sequence lengths");
+    if (Status s = ensure_weights(0, 0, stream); !s.ok()) return s;
+    if (Status s = set_lengths(stream); !s.ok()) return s;
     const int rc = hs_kv_evict(quant_type_ == KVQuantType::Fp8, k_codes_, v_codes_, k_scales_, v_scales_, &layout_, seq_lens_dev_, weights_,
                                weights_stride_, k_codes_, v_codes_, k_scales_, v_scales_, &layout_, seq_lens_dev_, weights_, weights_stride_,
                                nullptr, budget, sinks, recent, bound_ws_, bound_ws_bytes_, batch_, heads_, dim_, (int32_t)seq_pos, stream);
@@ -247,9 +255,9 @@ Status LayerKVCache::get_dense(void *keys_out, void *values_out, int dtype, hs_s
 Status LayerKVCache::decode_attention(const void *q, void *out, int32_t hq, float scale, hs_stream_t stream) {
     KVView v;
     if (Status s = get(&v); !s.ok()) return s;
-    if (Status s = ensure_scratch(hq, batch_, stream); !s.ok()) return s;
+    if (Status s = track_ ? ensure_weights(hq, 0, stream) : ensure_scratch(hq); !s.ok()) return s;
+    if (Status s = set_lengths(stream); !s.ok()) return s;
     if (track_) {
-        if (Status s = ensure_weights(hs_decode_weights_workspace_bytes(batch_, hq, heads_, dim_, (int32_t)max_seq_len), stream); !s.ok()) return s;
         return from_abi(hs_decode_step_weights(quant_type_ == KVQuantType::Fp8, q, nullptr, nullptr, HS_BF16, k_codes_, v_codes_, k_scales_,
                                                v_scales_, &layout_, seq_lens_dev_, out, weights_, weights_, weights_stride_, bound_ws_,
                                                bound_ws_bytes_, batch_, hq, heads_, dim_, (int32_t)seq_pos, scale, stream));
@@ -272,11 +280,11 @@ Status LayerKVCache::decode_step(const void *q, const void *k_new, const void *v
     }
     copy_upto_ = -1;  // the new token is not in the prompt copy
     seq_pos += 1;  // the entry point writes the new token at seq_pos - 1 and attends seq_pos tokens
-    Status s = ensure_scratch(hq, batch_, stream);
+    Status s = track_ ? ensure_weights(hq, 0, stream) : ensure_scratch(hq);
+    if (s.ok()) s = set_lengths(stream);
     int rc = HS_OK;
     if (s.ok() && track_) {
         if (!k_new || !v_new) s = err(HS_ERR_INVALID_ARGUMENT, "null buffer");
-        if (s.ok()) s = ensure_weights(hs_decode_weights_workspace_bytes(batch_, hq, heads_, dim_, (int32_t)max_seq_len), stream);
         if (s.ok()) s = clean_weights(seq_pos - 1, stream);
         if (s.ok())
             s = from_abi(hs_decode_step_weights(quant_type_ == KVQuantType::Fp8, q, k_new, v_new, dtype, k_codes_, v_codes_, k_scales_, v_scales_,
@@ -309,10 +317,8 @@ Status LayerKVCache::prefill(const void *q, const void *new_keys, const void *ne
     if (start_pos > seq_pos) return err(HS_ERR_INVALID_ARGUMENT, "start_pos is past the cached tokens");
     if (Status s = ensure_storage(batch, heads, dim); !s.ok()) return s;
     weights_dirty_ = std::max(weights_dirty_, seq_pos);
-    if (track_) {
-        const size_t ws = hs_attn_weights_workspace_bytes(batch, seq_len, hq, heads, dim, (int32_t)end_pos);
-        if (Status s = ensure_weights(ws, stream); !s.ok()) return s;
-    }
+    if (track_)
+        if (Status s = ensure_weights(hq, seq_len, stream); !s.ok()) return s;
     if (Status s = clean_weights(start_pos, stream); !s.ok()) return s;
     int rc;
     hs_kv_layout lay = layout_;

@@ -17,6 +17,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <string>
+#include <vector>
 
 #include "../../include/hs_attn.h"
 
@@ -105,8 +106,9 @@ class LayerKVCache {
 
   private:
     Status ensure_storage(int32_t batch, int32_t num_kv_heads, int32_t head_dim);
-    Status ensure_scratch(int32_t num_q_heads, int32_t batch, hs_stream_t stream);
-    Status ensure_weights(size_t workspace_bytes, hs_stream_t stream);
+    Status ensure_scratch(int32_t num_q_heads);
+    Status set_lengths(hs_stream_t stream);
+    Status ensure_weights(int32_t num_q_heads, int32_t seq_len, hs_stream_t stream);
     Status clean_weights(size_t from, hs_stream_t stream);
     void release();
 
@@ -127,6 +129,7 @@ class LayerKVCache {
     size_t weights_dirty_ = 0;
     void *bound_ws_ = nullptr;       // workspace of the weights' and the eviction's calls
     size_t bound_ws_bytes_ = 0;
+    std::vector<void *> outgrown_;   // earlier ones, freed with the storage
     // prompt scratch (enable_prompt_scratch)
     size_t prompt_tokens_ = 0;       // 0 = not enabled
     void *split_ws_ = nullptr, *copy_ = nullptr;

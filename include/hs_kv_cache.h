@@ -105,8 +105,10 @@ HS_API int hs_cache_prefill(hs_cache *c, const void *q, const void *new_keys, co
  *   and decode (hs_kv_layout.prefill_window, decode_window, attn_sinks); 0 = everything.
  * hs_cache_track_weights: from here on every attention call through the cache adds its softmax weights, summed over queries
  *   and over the query heads of a kv-head, to one fp32 entry per cached token (hs_decode_step_weights, hs_attn_weights).  A
- *   token starts at zero when it is cached; 0 stops and frees the entries.  The first counting call allocates them (run one
- *   before a graph capture, as for the workspace of a plain step).
+ *   token starts at zero when it is cached; 0 stops and frees the entries.  The first counting call, a prompt's or a
+ *   step's, allocates them and the workspace for max_seq_len tokens (run one before a graph capture, as for a plain step);
+ *   a later one allocates only for a longer chunk or more query heads, and what a captured step uses stays until the cache is
+ *   cleared.
  * hs_cache_get_weights: the entries as dense [batch, num_kv_heads, seq_pos], copied on `stream`.
  * hs_cache_evict: keeps `budget` tokens per (sequence, kv-head) -- the first `sinks`, the last `recent` and the heaviest of
  *   those between; without tracking the first `sinks` and the newest -- in place (hs_kv_evict).  seq_pos becomes

@@ -86,3 +86,72 @@ def test_view_carries_the_whole_window(early):
     cache.set_window(0)
     _, lay = _view(cache)
     assert (lay.prefill_window, lay.decode_window, lay.attn_sinks) == (0, 0, 0)
+
+
+def test_counted_prompt_allocates_once():
+    """A prompt in chunks: the buffers of a counting cache are those of the first chunk, at whatever position the others
+    are, and of the steps behind them.  (An unmeasured session comes first: the runtime's own memory for a kernel's first
+    launch shows in the same figure.)"""
+    B, S, T, Hq, Hkv, D = 1, 512, 16384, 32, 8, 128
+    q, k, v = bf16_randn(7200, B, S, Hq, D), bf16_randn(7201, B, S, Hkv, D), bf16_randn(7202, B, S, Hkv, D)
+    out = torch.empty_like(q)
+
+    def session():
+        cache, free = kc.LayerKVCache(T), []
+        cache.track_weights()
+        for at in range(0, 8192, S):
+            cache._check(kc.lib().hs_cache_prefill(cache._h, hb._ptr(q), hb._ptr(k), hb._ptr(v), hb._ptr(out), B, S, Hq, Hkv, D,
+                                                   ctypes.c_int64(at), ctypes.c_float(D ** -0.5), hb._stream()))
+            torch.cuda.synchronize()
+            free.append(torch.cuda.mem_get_info()[0])
+        for _ in range(2):
+            cache._check(kc.lib().hs_cache_decode_step(cache._h, hb._ptr(q), hb._ptr(k), hb._ptr(v), hb.HS_BF16, hb._ptr(out), Hq,
+                                                       ctypes.c_float(D ** -0.5), hb._stream()))
+            torch.cuda.synchronize()
+            free.append(torch.cuda.mem_get_info()[0])
+        cache.close()
+        return free
+
+    session()
+    free = session()
+    assert free == [free[0]] * len(free), free
+
+
+def test_captured_steps_outlive_longer_prompts():
+    """A counting step captured right behind a prompt (which has made the buffers) and replayed after a longer one, which
+    needs more: the step's buffers are still there, and every replay adds the same weights."""
+    Hq, Hkv, D, T, n = 8, 2, 128, 4096, 100
+    scale = D ** -0.5
+    q, k, v = bf16_randn(7250, 1, 1024, Hq, D), bf16_randn(7251, 1, 1024, Hkv, D), bf16_randn(7252, 1, 1024, Hkv, D)
+    qs, ks, vs = bf16_randn(7253, 1, Hq, D), bf16_randn(7254, 1, 1, Hkv, D), bf16_randn(7255, 1, 1, Hkv, D)
+    cache, plain = kc.LayerKVCache(T), kc.LayerKVCache(T)
+    out = torch.empty_like(qs)
+    for c in (cache, plain):
+        c.track_weights()
+        c.prefill(q[:, :n].contiguous(), k[:, :n], v[:, :n], 0, scale)
+
+    def step():
+        cache._check(kc.lib().hs_cache_decode_step(cache._h, hb._ptr(qs), hb._ptr(ks), hb._ptr(vs), hb.HS_BF16, hb._ptr(out), Hq,
+                                                   ctypes.c_float(scale), hb._stream()))
+
+    torch.cuda.synchronize()
+    g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=side):
+        step()
+    start = plain.weights()
+    want = plain.decode_step(qs, ks, vs, scale)
+    once = plain.weights()
+    for _ in range(3):  # the same step again and again: one more time its weights for every token
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    thrice = cache.weights()
+    add = once - torch.nn.functional.pad(start, (0, 1))
+    assert torch.allclose(thrice, once + 2 * add, rtol=1e-5, atol=0) and (add > 0).all()
+    cache.prefill(q, k, v, n + 1, scale)  # ten times as long
+    cache.truncate_to(n + 1)
+    before = cache.weights()
+    out.zero_()
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.allclose(cache.weights(), before + add, rtol=1e-5, atol=0)
