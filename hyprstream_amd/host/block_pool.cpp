@@ -130,6 +130,7 @@ PagedLayerKVCache::~PagedLayerKVCache() {
     clear();
     for (void *p : {(void *)table_dev_, (void *)len_dev_, (void *)head_scales_dev_, workspace_})
         if (p) (void)hipFree(p);
+    for (void *p : outgrown_) (void)hipFree(p);
     if (table_host_) (void)hipHostFree(table_host_);
     if (table_copied_) (void)hipEventDestroy(table_copied_);
 }
@@ -270,18 +271,15 @@ Status PagedLayerKVCache::get_dense(void *keys_out, void *values_out, int dtype,
     return from_abi(rc);
 }
 
+// An outgrown workspace is kept until the cache goes: queued work and captured steps may still use it.  (It at least
+// doubles, so those kept are no more than the one in use.)
 Status PagedLayerKVCache::grow_workspace(size_t bytes) {
     if (bytes <= workspace_bytes_) return {};
-    if (workspace_) {
-        if (hipError_t e = hipDeviceSynchronize(); e != hipSuccess) return hip_err(e, "waiting before the workspace grows");
-        (void)hipFree(workspace_);
-    }
-    workspace_ = nullptr;
-    workspace_bytes_ = 0;
-    if (hipError_t e = hipMalloc(&workspace_, bytes); e != hipSuccess) {
-        workspace_ = nullptr;
-        return hip_err(e, "allocating the workspace");
-    }
+    bytes = std::max(bytes, 2 * workspace_bytes_);
+    void *p = nullptr;
+    if (hipError_t e = hipMalloc(&p, bytes); e != hipSuccess) return hip_err(e, "allocating the workspace");
+    if (workspace_) outgrown_.push_back(workspace_);
+    workspace_ = p;
     workspace_bytes_ = bytes;
     return {};
 }
@@ -293,7 +291,7 @@ Status PagedLayerKVCache::evict(float *weights, int64_t weights_stride, int32_t 
     if ((size_t)budget >= seq_pos) return {};
     if (Status s = sync_table(stream); !s.ok()) return s;
     const int32_t heads = pool_->num_kv_heads(), dim = pool_->head_dim(), len = (int32_t)seq_pos;
-    if (Status s = grow_workspace(hs_kv_evict_workspace_bytes(1, heads, budget, len)); !s.ok()) return s;
+    if (Status s = grow_workspace(hs_kv_evict_workspace_bytes(1, heads, (int32_t)max_seq_len, len)); !s.ok()) return s;  // (sized once)
     if (hipError_t e = fill_i32(len_dev_, 1, len, (hipStream_t)stream); e != hipSuccess) return hip_err(e, "setting the length");
     const int32_t stride = (int32_t)((max_seq_len + kBlockSize - 1) / kBlockSize);
     const hs_kv_layout l = pool_->layout(table_dev_, table_dev_ + stride, stride);

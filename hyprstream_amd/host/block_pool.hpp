@@ -134,6 +134,7 @@ class PagedLayerKVCache {
     size_t mirror_high_ = 0;        // mirror entries below this index may still be read by an upload in flight
     void *workspace_ = nullptr;
     size_t workspace_bytes_ = 0;
+    std::vector<void *> outgrown_;  // earlier ones, freed with the cache
 };
 
 // One decode step over several paged caches of one pool (the batched path of the reference pads and concatenates

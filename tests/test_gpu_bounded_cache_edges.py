@@ -155,3 +155,31 @@ def test_captured_steps_outlive_longer_prompts():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want) and torch.allclose(cache.weights(), before + add, rtol=1e-5, atol=0)
+
+
+def test_captured_paged_steps_outlive_an_eviction():
+    """Attention over a paged cache, captured, and replayed after an eviction and new tokens have brought the cache back to
+    its length: the workspace that the eviction has outgrown is still there."""
+    Hq, Hkv, D, n = 4, 2, 64, 700
+    pool = kc.BlockPool(16, Hkv, D, kc.INT8)
+    cache = kc.PagedLayerKVCache(65536, pool, "s")
+    k, v, q = bf16_randn(7260, 1, n, Hkv, D), bf16_randn(7261, 1, n, Hkv, D), bf16_randn(7262, 1, Hq, D)
+    cache.update(k, v, 0)
+    first, out = cache.decode_attention(q, 0.125), torch.empty_like(q)
+    torch.cuda.synchronize()
+    g, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=side):
+        cache._check(kc.lib().hs_paged_cache_decode_attention(cache._h, hb._ptr(q), hb._ptr(out), Hq, ctypes.c_float(0.125), hb._stream()))
+    for _ in range(2):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, first)
+    cache.evict(300, 4, 100)
+    cache.update(k[:, :400], v[:, :400], 300)
+    second = cache.decode_attention(q, 0.125)
+    for _ in range(2):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, second) and not torch.equal(out, first)
