@@ -163,7 +163,7 @@ Status LayerKVCache::ensure_weights(int32_t hq, int32_t seq_len, hs_stream_t str
     return {};
 }
 
-// Tokens from `from` on are about to be cached anew: they start without weight.
+// Tokens from `from` on are cached anew (by a call that has not been refused): they start without weight.
 Status LayerKVCache::clean_weights(size_t from, hs_stream_t stream) {
     if (!weights_ || weights_dirty_ <= from) return {};
     const size_t to = weights_dirty_;
@@ -212,8 +212,6 @@ Status LayerKVCache::update(const void *new_keys, const void *new_values, int dt
     }
     if (Status s = ensure_storage(batch, heads, dim); !s.ok()) return s;
     copy_upto_ = -1;  // tokens written here are not in the prompt copy
-    weights_dirty_ = std::max(weights_dirty_, seq_pos);
-    if (Status s = clean_weights(start_pos, stream); !s.ok()) return s;
     int rc;
     if (quant_type_ == KVQuantType::Fp8) {
         if (start_pos == 0) {  // fresh prompt: calibrate the per-(sequence, head) scales on it
@@ -227,6 +225,8 @@ Status LayerKVCache::update(const void *new_keys, const void *new_values, int dt
                                  &layout_, nullptr, (int32_t)start_pos, batch, seq_len, heads, dim, stream);
     }
     if (rc != HS_OK) return from_abi(rc);
+    weights_dirty_ = std::max(weights_dirty_, seq_pos);
+    if (Status s = clean_weights(start_pos, stream); !s.ok()) return s;
     seq_pos = end_pos;
     return {};
 }
@@ -316,10 +316,8 @@ Status LayerKVCache::prefill(const void *q, const void *new_keys, const void *ne
     }
     if (start_pos > seq_pos) return err(HS_ERR_INVALID_ARGUMENT, "start_pos is past the cached tokens");
     if (Status s = ensure_storage(batch, heads, dim); !s.ok()) return s;
-    weights_dirty_ = std::max(weights_dirty_, seq_pos);
     if (track_)
         if (Status s = ensure_weights(hq, seq_len, stream); !s.ok()) return s;
-    if (Status s = clean_weights(start_pos, stream); !s.ok()) return s;
     int rc;
     hs_kv_layout lay = layout_;
     bool with_copy = false;
@@ -371,6 +369,8 @@ Status LayerKVCache::prefill(const void *q, const void *new_keys, const void *ne
     }
     copy_upto_ = rc == HS_OK && with_copy ? (int64_t)end_pos : -1;
     if (rc != HS_OK) return from_abi(rc);
+    weights_dirty_ = std::max(weights_dirty_, seq_pos);
+    if (Status s = clean_weights(start_pos, stream); !s.ok()) return s;
     seq_pos = end_pos;
     if (track_ && seq_len > 0) {
         rc = hs_attn_weights(quant_type_ == KVQuantType::Fp8, q, k_codes_, k_scales_, &lay, nullptr, (int32_t)start_pos, weights_, weights_,

@@ -183,3 +183,25 @@ def test_captured_paged_steps_outlive_an_eviction():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, second) and not torch.equal(out, first)
+
+
+def test_refused_calls_keep_the_weights():
+    """A call that is refused leaves the counted weights of the tokens it would have replaced as they are."""
+    B, S, Hq, Hkv, D = 1, 100, 4, 2, 64
+    cache = kc.LayerKVCache(256)
+    cache.track_weights()
+    q, k, v = bf16_randn(7300, B, S, Hq, D), bf16_randn(7301, B, S, Hkv, D), bf16_randn(7302, B, S, Hkv, D)
+    cache.prefill(q, k, v, 0, 0.125)
+    before = cache.weights()
+    assert (before > 0).all()
+    odd = bf16_randn(7303, B, 10, 3, D)  # three query heads over two kv-heads
+    with pytest.raises(kc.CacheError):
+        cache.prefill(odd, k[:, :10], v[:, :10], 40, 0.125)
+    rc = kc.lib().hs_cache_update(cache._h, hb._ptr(k), hb._ptr(v), 9, B, 10, Hkv, D, ctypes.c_int64(40), hb._stream())  # no such dtype
+    assert rc == hb.HS_ERR_INVALID_ARGUMENT
+    rc = kc.lib().hs_cache_update(cache._h, None, hb._ptr(v), hb.HS_BF16, B, 10, Hkv, D, ctypes.c_int64(40), hb._stream())
+    assert rc == hb.HS_ERR_INVALID_ARGUMENT
+    assert cache.seq_pos == S and torch.equal(cache.weights(), before)
+    cache.update(k[:, :10], v[:, :10], 40)  # one that is served: its tokens start without weight
+    after = cache.weights()
+    assert cache.seq_pos == 50 and torch.equal(after[:, :, :40], before[:, :, :40]) and not after[:, :, 40:].any()
