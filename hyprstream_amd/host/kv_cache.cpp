@@ -321,7 +321,7 @@ Status LayerKVCache::prefill(const void *q, const void *new_keys, const void *ne
     int rc;
     hs_kv_layout lay = layout_;
     bool with_copy = false;
-    if (prompt_tokens_ > 0) {
+    if (prompt_tokens_ > 0 && window_ == 0) {  // (a windowed call is neither split nor reads the copy)
         // key-split workspace: sized for the longest chunk seen (grows like the decode workspace)
         if (seq_len > split_tokens_) {
             if (split_ws_) {

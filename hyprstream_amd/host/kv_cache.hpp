@@ -78,7 +78,8 @@ class LayerKVCache {
     // first prefill after this call for max_prompt_tokens tokens, dropped by drop_prompt_scratch(), clear() and the
     // destructor).  The copy follows the prompt: a chunk at start_pos 0 begins it, a chunk that starts where the
     // last one ended extends it, and anything else written into the cache (update, decode_step) or taken out of it
-    // (truncate_to) retires it until the next prompt.  Results are those of prefill() without it within rounding.
+    // (truncate_to) retires it until the next prompt.  Results are those of prefill() without it within rounding.  A
+    // windowed cache takes neither.
     void enable_prompt_scratch(size_t max_prompt_tokens) { prompt_tokens_ = max_prompt_tokens; }
     void drop_prompt_scratch();
     bool prompt_copy_active() const { return copy_upto_ >= 0; }  // for tests: the next chunk would read the copy

@@ -127,7 +127,8 @@ HS_API int hs_cache_evict(hs_cache *c, int32_t budget, int32_t sinks, int32_t re
  * this call and freed by hs_cache_drop_prompt_scratch, hs_cache_clear and hs_cache_destroy.  It follows the prompt by
  * itself: a chunk at start_pos 0 begins it, a chunk that starts where the last one ended extends it, anything else
  * written into or cut from the cache (update, decode_step, truncate_to) retires it until the next prompt
- * (hs_cache_prompt_copy_active reports which).  max_prompt_tokens = 0 turns it off again. */
+ * (hs_cache_prompt_copy_active reports which).  Prompts of a windowed cache (hs_cache_set_window) read neither, and
+ * nothing is allocated or written for them.  max_prompt_tokens = 0 turns it off again. */
 HS_API void hs_cache_enable_prompt_scratch(hs_cache *c, int64_t max_prompt_tokens);
 HS_API void hs_cache_drop_prompt_scratch(hs_cache *c);
 HS_API int hs_cache_prompt_copy_active(const hs_cache *c);

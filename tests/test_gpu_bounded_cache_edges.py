@@ -205,3 +205,28 @@ def test_refused_calls_keep_the_weights():
     cache.update(k[:, :10], v[:, :10], 40)  # one that is served: its tokens start without weight
     after = cache.weights()
     assert cache.seq_pos == 50 and torch.equal(after[:, :, :40], before[:, :, :40]) and not after[:, :, 40:].any()
+
+
+@pytest.mark.parametrize("quant", [kc.INT8, kc.FP8])
+def test_windowed_prompt_keeps_no_copy(quant):
+    """The prompt scratch serves prompts without a window: a windowed one is neither copied nor split, so nothing is
+    allocated or written for it."""
+    B, S, Hq, Hkv, D, cap = 1, 512, 32, 8, 128, 65536
+    q, k, v = bf16_randn(7400, B, S, Hq, D), bf16_randn(7401, B, S, Hkv, D), bf16_randn(7402, B, S, Hkv, D)
+    cache, plain = kc.LayerKVCache(cap, quant), kc.LayerKVCache(cap, quant)
+    for c in (cache, plain):
+        c.set_window(300, 4)
+        c.update(k[:, :64], v[:, :64], 0)  # the storage
+    cache.enable_prompt_scratch(cap)
+    out, ref = cache.prefill(q, k, v, 0, D ** -0.5), plain.prefill(q, k, v, 0, D ** -0.5)
+    out = cache.prefill(q, k, v, 0, D ** -0.5)
+    assert not cache.prompt_copy_active and torch.equal(out, ref)
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    cache.drop_prompt_scratch()
+    assert torch.cuda.mem_get_info()[0] == free
+    assert torch.equal(cache.prefill(q, k, v, S, D ** -0.5), plain.prefill(q, k, v, S, D ** -0.5))
+    cache.set_window(0)  # and without one it is begun by a prompt at position 0
+    plain.set_window(0)
+    cache.prefill(q, k, v, 0, D ** -0.5)
+    assert cache.prompt_copy_active
