@@ -200,6 +200,7 @@ extern "C" {
     pub fn hs_paged_cache_prefill(c: *mut hs_paged_cache, q: *const c_void, new_keys: *const c_void, new_values: *const c_void, out: *mut c_void, seq_len: i32, num_q_heads: i32, start_pos: i64, softmax_scale: f32, stream: hs_stream_t) -> c_int;
     pub fn hs_paged_cache_clear(c: *mut hs_paged_cache);
     pub fn hs_paged_cache_truncate_to(c: *mut hs_paged_cache, pos: i64);
+    pub fn hs_paged_cache_get_view(c: *mut hs_paged_cache, k_codes: *mut *mut c_void, v_codes: *mut *mut c_void, k_scales: *mut *mut f32, v_scales: *mut *mut f32, layout: *mut hs_kv_layout, stream: hs_stream_t) -> c_int;
     pub fn hs_paged_cache_evict(c: *mut hs_paged_cache, weights: *mut f32, weights_stride: i64, budget: i32, sinks: i32, recent: i32, stream: hs_stream_t) -> c_int;
     pub fn hs_paged_cache_seq_pos(c: *const hs_paged_cache) -> i64;
     pub fn hs_paged_cache_num_blocks(c: *const hs_paged_cache) -> i64;

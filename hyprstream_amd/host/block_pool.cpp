@@ -256,6 +256,19 @@ Status PagedLayerKVCache::prefill(const void *q, const void *new_keys, const voi
     return {};
 }
 
+Status PagedLayerKVCache::get(KVView *v, hs_stream_t stream) {
+    if (seq_pos == 0) return err(HS_ERR_INVALID_ARGUMENT, "Cache is empty");
+    if (Status s = sync_table(stream); !s.ok()) return s;
+    const int32_t stride = (int32_t)((max_seq_len + kBlockSize - 1) / kBlockSize);
+    v->k_codes = v->v_codes = pool_->codes();
+    v->k_scales = pool_->fp8() ? head_scales_dev_ : pool_->scales();
+    v->v_scales = pool_->fp8() ? head_scales_dev_ + pool_->num_kv_heads() : pool_->scales();
+    v->layout = pool_->layout(table_dev_, table_dev_ + stride, stride);
+    v->batch = 1; v->seq_pos = (int32_t)seq_pos; v->num_kv_heads = pool_->num_kv_heads(); v->head_dim = pool_->head_dim();
+    v->quant_type = pool_->format();
+    return {};
+}
+
 Status PagedLayerKVCache::get_dense(void *keys_out, void *values_out, int dtype, hs_stream_t stream) {
     if (seq_pos == 0) return err(HS_ERR_INVALID_ARGUMENT, "Cache is empty");
     if (Status s = sync_table(stream); !s.ok()) return s;

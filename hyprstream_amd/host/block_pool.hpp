@@ -97,6 +97,7 @@ class PagedLayerKVCache {
     Status update(const void *new_keys, const void *new_values, int dtype, int32_t seq_len, size_t start_pos,
                   hs_stream_t stream = nullptr);
     Status get_dense(void *keys_out, void *values_out, int dtype, hs_stream_t stream = nullptr);
+    Status get(KVView *v, hs_stream_t stream = nullptr);  // the sequence through its block table
     Status decode_attention(const void *q, void *out, int32_t num_q_heads, float softmax_scale, hs_stream_t stream = nullptr);
     // update(seq_len bf16 tokens at start_pos) + causal attention of those tokens over [cached history | themselves];
     // q, out: bf16 [1, seq_len, num_q_heads, head_dim].  Blocks are taken as in update().

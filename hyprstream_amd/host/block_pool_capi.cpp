@@ -102,6 +102,18 @@ int hs_paged_cache_prefill(hs_paged_cache *c, const void *q, const void *new_key
 }
 void hs_paged_cache_clear(hs_paged_cache *c) { if (c) c->cache.clear(); }
 void hs_paged_cache_truncate_to(hs_paged_cache *c, int64_t pos) { if (c && pos >= 0) c->cache.truncate_to((size_t)pos); }
+int hs_paged_cache_get_view(hs_paged_cache *c, void **k_codes, void **v_codes, float **k_scales, float **v_scales,
+                            hs_kv_layout *layout, hs_stream_t stream) {
+    if (!c) return HS_ERR_INVALID_ARGUMENT;
+    hs::KVView v;
+    if (const int rc = c->done(c->cache.get(&v, stream))) return rc;
+    if (k_codes) *k_codes = v.k_codes;
+    if (v_codes) *v_codes = v.v_codes;
+    if (k_scales) *k_scales = v.k_scales;
+    if (v_scales) *v_scales = v.v_scales;
+    if (layout) *layout = v.layout;
+    return HS_OK;
+}
 int hs_paged_cache_evict(hs_paged_cache *c, float *weights, int64_t weights_stride, int32_t budget, int32_t sinks, int32_t recent,
                          hs_stream_t stream) {
     if (!c) return HS_ERR_INVALID_ARGUMENT;

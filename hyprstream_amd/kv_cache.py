@@ -21,7 +21,7 @@ EXPORTS = [
     "hs_pool_create", "hs_pool_create_format", "hs_pool_quant_type", "hs_pool_destroy", "hs_pool_last_error", "hs_pool_allocate", "hs_pool_free", "hs_pool_owner_of",
     "hs_pool_used_blocks", "hs_pool_free_block_count", "hs_pool_total_blocks", "hs_pool_used_memory",
     "hs_paged_cache_create", "hs_paged_cache_destroy", "hs_paged_cache_last_error", "hs_paged_cache_update",
-    "hs_paged_cache_get_dense", "hs_paged_cache_decode_attention", "hs_paged_cache_clear", "hs_paged_cache_truncate_to", "hs_paged_cache_evict",
+    "hs_paged_cache_get_dense", "hs_paged_cache_decode_attention", "hs_paged_cache_clear", "hs_paged_cache_truncate_to", "hs_paged_cache_get_view", "hs_paged_cache_evict",
     "hs_paged_cache_seq_pos", "hs_paged_cache_num_blocks", "hs_paged_batch_decode_step",
     "hs_compat_create", "hs_compat_destroy", "hs_compat_set_uint", "hs_compat_set_opt_uint", "hs_compat_set_str",
     "hs_compat_add_layer_type", "hs_compat_set_rope_scaling", "hs_compat_set_kv_quant",
@@ -280,6 +280,16 @@ class BlockPool(_Handle):
         return lib().hs_pool_used_memory(self._h)
 
 
+class _Buffer:
+    """A device address where the bindings take a tensor."""
+
+    def __init__(self, address):
+        self._address = address
+
+    def data_ptr(self):
+        return self._address
+
+
 class PagedLayerKVCache(_Handle):
     """LayerKVCache::new_paged (kv_cache.rs:1100-1120): one sequence, int8 blocks from a shared pool."""
 
@@ -340,6 +350,14 @@ class PagedLayerKVCache(_Handle):
 
     def truncate_to(self, pos):
         lib().hs_paged_cache_truncate_to(self._h, ctypes.c_int64(pos))
+
+    def view(self):
+        """([k_codes, v_codes, k_scales, v_scales], layout) of the cache's one sequence, for the calls of bindings that
+        attend or count (decode_step_weights without a new token, attn_weights, ...).  It stays good while tokens come
+        in by update and prefill; ask again behind a batch step."""
+        p, layout = [ctypes.c_void_p() for _ in range(4)], hb.KvLayout()
+        self._check(lib().hs_paged_cache_get_view(self._h, *[ctypes.byref(x) for x in p], ctypes.byref(layout), hb._stream()))
+        return [_Buffer(x.value) for x in p], layout
 
     def evict(self, budget, sinks=0, recent=0, weights=None):
         """Keep `budget` tokens per kv-head and give the blocks behind them back; weights: fp32 [Hkv, stride], moved along."""

@@ -182,9 +182,16 @@ HS_API int hs_paged_cache_prefill(hs_paged_cache *c, const void *q, const void *
                                   hs_stream_t stream);
 HS_API void hs_paged_cache_clear(hs_paged_cache *c);
 HS_API void hs_paged_cache_truncate_to(hs_paged_cache *c, int64_t pos);
+/* The cache's one sequence as the entry points of hs_attn.h take it: codes, scales (of the pool; fp8: the cache's own head
+ * scales) and the paged layout.  The addresses stay as long as the cache; the block table behind them is brought up to date
+ * on `stream` by this call and by the cache's own update, prefill and attention (not by a batch step, which takes tables of
+ * its own: ask again behind one).  What is cached through the view is not known to the cache: tokens come in by update and
+ * prefill.  Fails with "Cache is empty" when seq_pos == 0. */
+HS_API int hs_paged_cache_get_view(hs_paged_cache *c, void **k_codes, void **v_codes, float **k_scales, float **v_scales,
+                                   hs_kv_layout *layout, hs_stream_t stream);
 /* Keeps `budget` tokens per kv-head in place, as hs_cache_evict does, and gives the blocks behind them back to the pool.
- * weights: device fp32 [num_kv_heads, weights_stride], one entry per cached token (hs_decode_step_weights and
- * hs_attn_weights on the cache's block table fill such rows), moved with the tokens that stay; NULL = the first `sinks` and
+ * weights: device fp32 [num_kv_heads, weights_stride], one entry per cached token (hs_decode_step_weights, without a new
+ * token, and hs_attn_weights on hs_paged_cache_get_view's layout fill such rows), moved with the tokens that stay; NULL = the first `sinks` and
  * the newest.  As after hs_paged_cache_truncate_to, work queued on other streams must not still read the blocks. */
 HS_API int hs_paged_cache_evict(hs_paged_cache *c, float *weights, int64_t weights_stride, int32_t budget, int32_t sinks,
                                 int32_t recent, hs_stream_t stream);

@@ -230,3 +230,62 @@ def test_windowed_prompt_keeps_no_copy(quant):
     plain.set_window(0)
     cache.prefill(q, k, v, 0, D ** -0.5)
     assert cache.prompt_copy_active
+
+
+# ---- the paged mirror
+@pytest.mark.parametrize("quant", [kc.INT8, kc.FP8])
+def test_counted_session_over_a_paged_cache(quant):
+    """A counted session over a paged cache, its weights made through the view, against the contiguous mirror's own
+    counting: outputs, weights and the tokens that an eviction leaves, bit for bit."""
+    Hq, Hkv, D, cap, fp8 = 8, 2, 128, 1500, quant == kc.FP8
+    scale = D ** -0.5
+    pool = kc.BlockPool(16, Hkv, D, quant)
+    paged, plain, other = kc.PagedLayerKVCache(cap, pool, "a"), kc.LayerKVCache(cap, quant), kc.PagedLayerKVCache(cap, pool, "b")
+    with pytest.raises(kc.CacheError, match="empty"):
+        paged.view()
+    plain.track_weights()
+    stride = (cap + 3) // 4 * 4
+    w = torch.zeros(1, Hkv, stride, device=DEV)
+    ws = _space(max(hb.attn_weights_workspace_bytes(1, 700, Hq, Hkv, D, cap), hb.decode_weights_workspace_bytes(1, Hq, Hkv, D, cap)))
+    seed = [7600]
+
+    def rnd(*s):
+        seed[0] += 1
+        return bf16_randn(seed[0], *s)
+
+    def same():
+        n = plain.seq_pos
+        assert paged.seq_pos == n and torch.equal(w[:, :, :n], plain.weights())
+        assert all(torch.equal(a, b) for a, b in zip(paged.get(torch.float32), plain.get(torch.float32)))
+
+    def chunk(S, at):
+        q, k, v = rnd(1, S, Hq, D), rnd(1, S, Hkv, D), rnd(1, S, Hkv, D)
+        assert torch.equal(paged.prefill(q, k, v, at, scale), plain.prefill(q, k, v, at, scale))
+        buffers, layout = paged.view()
+        w[:, :, at:] = 0
+        hb.attn_weights(q, buffers[0], buffers[2], layout, w, w, ws, Hkv, at + S, scale, start_pos=at, fp8=fp8)
+        same()
+
+    def step(buffers, layout):
+        q, k, v = rnd(1, Hq, D), rnd(1, 1, Hkv, D), rnd(1, 1, Hkv, D)
+        n, out = paged.seq_pos, torch.empty_like(q)
+        paged.update(k, v, n)
+        w[:, :, n] = 0
+        lens = torch.full((1,), n + 1, dtype=torch.int32, device=DEV)
+        hb.decode_step_weights(q, None, None, *buffers, layout, lens, out, w, w, ws, Hkv, n + 1, scale, fp8=fp8)
+        assert torch.equal(out, plain.decode_step(q, k, v, scale))
+        same()
+
+    other.update(rnd(1, 10, Hkv, D), rnd(1, 10, Hkv, D), 0)  # its blocks lie between the session's
+    chunk(700, 0)
+    other.update(rnd(1, 300, Hkv, D), rnd(1, 300, Hkv, D), 10)
+    chunk(60, 700)
+    view = paged.view()
+    for _ in range(12):  # over a block's end, through one view
+        step(*view)
+    for c in (paged, plain):
+        c.evict(300, 4, 100, **({"weights": w[0]} if c is paged else {}))
+    same()
+    for _ in range(3):
+        step(*view)
+    chunk(500, paged.seq_pos)
