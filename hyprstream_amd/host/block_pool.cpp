@@ -40,6 +40,7 @@ BlockPool::BlockPool(size_t num_blocks, int32_t heads, int32_t dim, KVQuantType 
     free_list_.reserve(num_blocks);
     for (size_t id = 0; id < num_blocks; ++id) free_list_.push_back((BlockId)id);  // pop() hands out the highest id first
     owner_.resize(num_blocks);
+    fence_.resize(num_blocks);
 }
 
 BlockPool::~BlockPool() {
@@ -57,7 +58,7 @@ Status BlockPool::allocate(const CacheOwner &owner, BlockId *id) {
     return {};
 }
 
-Status BlockPool::free(const CacheOwner &owner, BlockId id) {
+Status BlockPool::free(const CacheOwner &owner, BlockId id, std::shared_ptr<BlockFence> until) {
     std::lock_guard<std::mutex> g(mu_);
     if (id < 0 || (size_t)id >= total_) return err(HS_ERR_INVALID_ARGUMENT, "Invalid block ID: " + std::to_string(id));
     const auto &cur = owner_[(size_t)id];
@@ -66,8 +67,40 @@ Status BlockPool::free(const CacheOwner &owner, BlockId id) {
         return err(HS_ERR_INVALID_ARGUMENT, "cross-owner block free rejected: block " + std::to_string(id) + " owned by " +
                                                 cur->str() + ", freed by " + owner.str());
     owner_[(size_t)id].reset();
+    if (until) fence_[(size_t)id] = std::move(until);  // (queued behind an earlier one that was still there)
     free_list_.push_back(id);
     return {};
+}
+
+Status BlockPool::await(BlockId id, hs_stream_t stream, bool *clear) {
+    std::lock_guard<std::mutex> g(mu_);
+    auto &f = fence_[(size_t)id];
+    *clear = !f;
+    if (*clear) return {};
+    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+    if (hipError_t e = hipStreamIsCapturing((hipStream_t)stream, &capturing); e != hipSuccess) return hip_err(e, "asking for a capture");
+    if (capturing != hipStreamCaptureStatusNone)
+        return err(HS_ERR_BUSY, "a block comes from an eviction that is still queued: make one call with it before the capture");
+    hipError_t e = hipEventQuery(f->event);
+    if (e == hipSuccess) {
+        f.reset();
+        *clear = true;
+        return {};
+    }
+    if (e == hipErrorNotReady) {
+        (void)hipGetLastError();  // (not an error of the launches behind it)
+        e = hipStreamWaitEvent((hipStream_t)stream, f->event, 0);
+    }
+    return hip_err(e, "waiting for a block");
+}
+
+Status BlockPool::await_host(BlockId id) {
+    std::shared_ptr<BlockFence> f;
+    {
+        std::lock_guard<std::mutex> g(mu_);
+        f = std::move(fence_[(size_t)id]);
+    }
+    return f ? hip_err(hipEventSynchronize(f->event), "waiting for a block") : Status{};
 }
 
 const CacheOwner *BlockPool::owner_of(BlockId id) const {
@@ -151,6 +184,18 @@ Status PagedLayerKVCache::reserve(size_t end_pos) {
     return {};
 }
 
+Status PagedLayerKVCache::await_blocks(hs_stream_t stream) {
+    bool all = true;
+    for (size_t i = awaited_; i < key_blocks_.size(); ++i)
+        for (BlockId id : {key_blocks_[i], value_blocks_[i]}) {
+            bool clear;
+            if (Status s = pool_->await(id, stream, &clear); !s.ok()) return s;
+            all = all && clear;
+        }
+    if (all) awaited_ = key_blocks_.size();
+    return {};
+}
+
 // New table entries (a block pair every 256 tokens) go to the device with a copy ordered on the caller's stream, so
 // a kernel of an earlier step on that stream never sees a table that changes under it.  The copy's source is a
 // pinned mirror of the table (a copy from pageable std::vector storage is staged by the runtime, blocks the host and
@@ -158,6 +203,7 @@ Status PagedLayerKVCache::reserve(size_t end_pos) {
 // reading; only after blocks were returned (clear / truncate_to) are entries rewritten, and then the last copy's
 // event is waited for first.
 Status PagedLayerKVCache::sync_table(hs_stream_t stream) {
+    if (Status s = await_blocks(stream); !s.ok()) return s;
     const size_t max_blocks = std::max<size_t>((max_seq_len + kBlockSize - 1) / kBlockSize, 1);
     hipError_t e;
     if (!table_dev_) {
@@ -302,6 +348,10 @@ Status PagedLayerKVCache::evict(float *weights, int64_t weights_stride, int32_t 
     if (budget <= 0 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
         return err(HS_ERR_INVALID_ARGUMENT, "need budget > 0 and 0 <= sinks + recent <= budget");
     if ((size_t)budget >= seq_pos) return {};
+    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+    if (hipError_t e = hipStreamIsCapturing((hipStream_t)stream, &capturing); e != hipSuccess) return hip_err(e, "asking for a capture");
+    if (capturing != hipStreamCaptureStatusNone)
+        return err(HS_ERR_INVALID_ARGUMENT, "a paged cache is not evicted under stream capture: its blocks go back to the pool once");
     if (Status s = sync_table(stream); !s.ok()) return s;
     const int32_t heads = pool_->num_kv_heads(), dim = pool_->head_dim(), len = (int32_t)seq_pos;
     if (Status s = grow_workspace(hs_kv_evict_workspace_bytes(1, heads, (int32_t)max_seq_len, len)); !s.ok()) return s;  // (sized once)
@@ -313,7 +363,15 @@ Status PagedLayerKVCache::evict(float *weights, int64_t weights_stride, int32_t 
                                pool_->codes(), pool_->codes(), ks, vs, &l, len_dev_, weights, weights_stride, nullptr, budget, sinks,
                                recent, workspace_, workspace_bytes_, 1, heads, dim, len, stream);
     if (rc != HS_OK) return from_abi(rc);
-    truncate_to((size_t)budget);
+    // the blocks go back now, the eviction that reads them is only queued: their next owner waits for it
+    auto fence = std::make_shared<BlockFence>();
+    hipError_t e = hipEventCreateWithFlags(&fence->event, hipEventDisableTiming);
+    if (e == hipSuccess) e = hipEventRecord(fence->event, (hipStream_t)stream);
+    if (e != hipSuccess) {
+        fence.reset();
+        if ((e = hipStreamSynchronize((hipStream_t)stream)) != hipSuccess) return hip_err(e, "waiting for the eviction");
+    }
+    give_back((size_t)budget, fence);
     return {};
 }
 
@@ -341,19 +399,22 @@ void PagedLayerKVCache::clear() {
     for (BlockId id : value_blocks_) (void)pool_->free(owner_, id);
     key_blocks_.clear();
     value_blocks_.clear();
-    table_synced_ = 0;
+    table_synced_ = awaited_ = 0;
     seq_pos = 0;
 }
 
-void PagedLayerKVCache::truncate_to(size_t pos) {
+void PagedLayerKVCache::truncate_to(size_t pos) { give_back(pos, nullptr); }
+
+void PagedLayerKVCache::give_back(size_t pos, const std::shared_ptr<BlockFence> &until) {
     if (pos >= seq_pos) return;
     const size_t needed = pos == 0 ? 0 : (pos - 1) / kBlockSize + 1;
     if (key_blocks_.size() > needed) {
-        for (size_t i = needed; i < key_blocks_.size(); ++i) (void)pool_->free(owner_, key_blocks_[i]);
-        for (size_t i = needed; i < value_blocks_.size(); ++i) (void)pool_->free(owner_, value_blocks_[i]);
+        for (size_t i = needed; i < key_blocks_.size(); ++i) (void)pool_->free(owner_, key_blocks_[i], until);
+        for (size_t i = needed; i < value_blocks_.size(); ++i) (void)pool_->free(owner_, value_blocks_[i], until);
         key_blocks_.resize(needed);
         value_blocks_.resize(needed);
         table_synced_ = std::min(table_synced_, needed);
+        awaited_ = std::min(awaited_, needed);
     }
     seq_pos = pos;
 }
@@ -411,6 +472,8 @@ Status PagedBatch::decode_step(PagedLayerKVCache *const *rows, int32_t n, const 
         stride = std::max(stride, rows[i]->num_blocks());
     }
     if (Status s = pool_->ensure_device(); !s.ok()) return s;
+    for (int32_t i = 0; i < n; ++i)
+        if (Status s = rows[i]->await_blocks(stream); !s.ok()) return s;
     // int32 units of the slot: K tables, V tables, lengths; an fp8 step adds (8-byte aligned) the rows' scale pointers
     // and the gathered [2][n][Hkv] scales
     const bool fp8 = pool_->fp8();

@@ -39,6 +39,14 @@ struct CacheOwner {
     std::string str() const;
 };
 
+// Queued work that still touches blocks their owner has given back.
+struct BlockFence {
+    hipEvent_t event = nullptr;
+    ~BlockFence() {
+        if (event) (void)hipEventDestroy(event);
+    }
+};
+
 class BlockPool {
   public:
     // format: Int8 (codes + per-token scales in every block) or Fp8 (e4m3fn codes only; the per-(sequence, kv-head)
@@ -53,7 +61,12 @@ class BlockPool {
     // into admission-defer.
     Status allocate(const CacheOwner &owner, BlockId *id);
     // Returns a block.  A block of another owner, a free block or an invalid id is refused and nothing changes.
-    Status free(const CacheOwner &owner, BlockId id);
+    // `until`: work queued when the block is given back; its next owner awaits it.
+    Status free(const CacheOwner &owner, BlockId id, std::shared_ptr<BlockFence> until = nullptr);
+    // Orders work on `stream` behind the fence of a block that its new owner is about to use.  *clear: there is none any
+    // more (until then other streams of the owner have to ask as well).  A capturing stream cannot wait: HS_ERR_BUSY.
+    Status await(BlockId id, hs_stream_t stream, bool *clear);
+    Status await_host(BlockId id);  // the same for an owner without a stream: blocks
     const CacheOwner *owner_of(BlockId id) const;  // nullptr when free or invalid
     size_t used_blocks() const;
     size_t free_block_count() const;
@@ -79,6 +92,7 @@ class BlockPool {
     KVQuantType format_;
     std::vector<BlockId> free_list_;
     std::vector<std::unique_ptr<CacheOwner>> owner_;
+    std::vector<std::shared_ptr<BlockFence>> fence_;
     int8_t *codes_ = nullptr;
     float *scales_ = nullptr;
 };
@@ -107,6 +121,8 @@ class PagedLayerKVCache {
     void truncate_to(size_t pos);  // frees the blocks beyond the last needed one (kv_cache.rs:1725-1748)
     // Keep `budget` tokens per kv-head (hs_kv_evict in place) and give the blocks behind them back to the pool.  weights:
     // device [num_kv_heads, weights_stride], the kept tokens' entries moved with them; nullptr = the sinks and the newest.
+    // The blocks' next owner waits for the eviction on the GPU (await).  Not under stream capture: blocks go back once, when
+    // the call is made, and a graph would move tokens whenever it is replayed.
     Status evict(float *weights, int64_t weights_stride, int32_t budget, int32_t sinks, int32_t recent, hs_stream_t stream = nullptr);
     size_t num_blocks() const { return key_blocks_.size(); }
     const std::vector<BlockId> &key_blocks() const { return key_blocks_; }
@@ -120,8 +136,12 @@ class PagedLayerKVCache {
     size_t seq_pos = 0;
     size_t max_seq_len = 0;
 
+    // Orders work on `stream` behind what former owners of the cache's blocks still have queued (sync_table does it, too).
+    Status await_blocks(hs_stream_t stream);
+
   private:
     Status sync_table(hs_stream_t stream);
+    void give_back(size_t pos, const std::shared_ptr<BlockFence> &until);
     Status grow_workspace(size_t bytes);
     std::shared_ptr<BlockPool> pool_;
     CacheOwner owner_;
@@ -131,6 +151,7 @@ class PagedLayerKVCache {
     float *head_scales_dev_ = nullptr;  // fp8 pools: [2][Hkv], K then V, calibrated by the update at start_pos 0
     int32_t *table_host_ = nullptr; // pinned mirror of the table, the source of the uploads
     hipEvent_t table_copied_ = nullptr;  // recorded behind the last upload
+    size_t awaited_ = 0;            // block pairs no former owner's work touches any more
     size_t table_synced_ = 0;       // number of blocks the device table already holds
     size_t mirror_high_ = 0;        // mirror entries below this index may still be read by an upload in flight
     void *workspace_ = nullptr;

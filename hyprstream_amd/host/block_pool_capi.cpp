@@ -53,7 +53,9 @@ const char *hs_pool_last_error(const hs_pool *p) { return p ? p->last_error.c_st
 
 int hs_pool_allocate(hs_pool *p, int kind, uint64_t id, const char *name, int32_t *block_id) {
     if (!p || !block_id) return HS_ERR_INVALID_ARGUMENT;
-    return p->done(p->pool->allocate(owner(kind, id, name), block_id));
+    hs::Status s = p->pool->allocate(owner(kind, id, name), block_id);
+    if (s.ok()) s = p->pool->await_host(*block_id);  // (its user's streams are not known here)
+    return p->done(s);
 }
 int hs_pool_free(hs_pool *p, int kind, uint64_t id, const char *name, int32_t block_id) {
     if (!p) return HS_ERR_INVALID_ARGUMENT;

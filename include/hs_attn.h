@@ -63,7 +63,8 @@ enum hs_status {
     HS_ERR_WORKSPACE = 3,        /* workspace too small */
     HS_ERR_LAUNCH = 4,           /* hipGetLastError() after the launch */
     HS_ERR_POOL_EXHAUSTED = 5,   /* host-side block pool has no free block (fail-soft, hs_kv_cache.h) */
-    HS_ERR_BUSY = 6              /* hs_decode_attn_int8_static: the GPU's built-in scratch is in use on another stream */
+    HS_ERR_BUSY = 6              /* hs_decode_attn_int8_static: the GPU's built-in scratch is in use on another stream; a
+                                    captured call over pool blocks that a queued eviction still reads (hs_kv_cache.h) */
 };
 
 enum hs_dtype { HS_BF16 = 0, HS_F32 = 1, HS_F16 = 2 };

@@ -192,7 +192,9 @@ HS_API int hs_paged_cache_get_view(hs_paged_cache *c, void **k_codes, void **v_c
 /* Keeps `budget` tokens per kv-head in place, as hs_cache_evict does, and gives the blocks behind them back to the pool.
  * weights: device fp32 [num_kv_heads, weights_stride], one entry per cached token (hs_decode_step_weights, without a new
  * token, and hs_attn_weights on hs_paged_cache_get_view's layout fill such rows), moved with the tokens that stay; NULL = the first `sinks` and
- * the newest.  As after hs_paged_cache_truncate_to, work queued on other streams must not still read the blocks. */
+ * the newest.  The eviction is only queued when the call returns: whoever takes the blocks next waits for it (caches on the
+ * GPU, on the stream of their first calls with them; hs_pool_allocate on the host).  Other work that still reads this cache
+ * has to be ordered by the caller, as for hs_paged_cache_truncate_to and _clear.  Refused under stream capture. */
 HS_API int hs_paged_cache_evict(hs_paged_cache *c, float *weights, int64_t weights_stride, int32_t budget, int32_t sinks,
                                 int32_t recent, hs_stream_t stream);
 HS_API int64_t hs_paged_cache_seq_pos(const hs_paged_cache *c);

@@ -289,3 +289,74 @@ def test_counted_session_over_a_paged_cache(quant):
     for _ in range(3):
         step(*view)
     chunk(500, paged.seq_pos)
+
+
+@pytest.mark.parametrize("taker", ["update", "prefill", "batch", "pool", "clear"])
+def test_blocks_of_a_queued_eviction_wait_for_it(taker):
+    """An eviction is still queued behind other work of its stream when another session, on a stream of its own, is given
+    the blocks behind the kept tokens: neither reads or overwrites what the other holds."""
+    Hq, Hkv, D, n = 4, 2, 128, 1024
+    pool = kc.BlockPool(10, Hkv, D, kc.INT8)
+    one, two, ref = kc.PagedLayerKVCache(2048, pool, "one"), kc.PagedLayerKVCache(2048, pool, "two"), kc.LayerKVCache(2048)
+    k, v = bf16_randn(7700, 1, n, Hkv, D), bf16_randn(7701, 1, n, Hkv, D)
+    k2, v2, q2 = bf16_randn(7702, 1, 257, Hkv, D), bf16_randn(7703, 1, 257, Hkv, D), bf16_randn(7704, 1, 257, Hq, D)
+    two.update(k2[:, :256], v2[:, :256], 0)
+    for c in (one, ref):  # twice: the first time makes the workspaces
+        c.update(k, v, 0)
+        c.evict(300, 4, 100)
+        c.update(k[:, 300:], v[:, 300:], 300)
+    assert pool.free_block_count() == 0
+    big = torch.randn(8192, 8192, device=DEV)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s1):
+        for _ in range(10):
+            big = big @ big * 1e-4
+        one.evict(300, 4, 100)
+    busy = not s1.query()
+    assert pool.free_block_count() == 4
+    third = kc.PagedLayerKVCache(2048, pool, "three")
+    with torch.cuda.stream(s2):
+        if taker == "update":
+            two.update(k2[:, 256:], v2[:, 256:], 256)
+        elif taker == "prefill":
+            two.prefill(q2[:, 256:], k2[:, 256:], v2[:, 256:], 256, 0.1)
+        elif taker == "batch":
+            kc.paged_batch_decode_step(pool, [two], q2[:, 256].contiguous(), k2[:, 256:].contiguous(), v2[:, 256:].contiguous(), 0.1)
+        elif taker == "pool":
+            ids = [pool.allocate("raw") for _ in range(4)]
+            assert s1.query() and pool.free_block_count() == 0
+            for i in ids:
+                pool.free("raw", i)
+        else:  # taken, never used and given back: the next owner still waits
+            third.update(k2[:, :1], v2[:, :1], 0)
+            third.clear()
+            two.update(k2[:, 256:], v2[:, 256:], 256)
+        if taker not in ("batch", "pool"):
+            assert busy and not s1.query()  # the host has not waited
+    torch.cuda.synchronize()
+    ref.evict(300, 4, 100)
+    assert all(torch.equal(a, b) for a, b in zip(one.get(torch.float32), ref.get(torch.float32)))
+    if taker != "pool":
+        alone = kc.LayerKVCache(2048)
+        alone.update(k2, v2, 0)
+        assert two.seq_pos == 257 and all(torch.equal(a, b) for a, b in zip(two.get(torch.float32), alone.get(torch.float32)))
+
+
+def test_paged_eviction_is_refused_under_capture():
+    pool = kc.BlockPool(8, 2, 64, kc.INT8)
+    cache = kc.PagedLayerKVCache(1024, pool, "s")
+    k = bf16_randn(7750, 1, 600, 2, 64)
+    cache.update(k, k, 0)
+    before = [t.clone() for t in cache.get(torch.float32)]
+    x = torch.zeros(4, device=DEV)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+        with pytest.raises(kc.CacheError, match="capture"):
+            cache.evict(100)
+        x += 1
+    g.replay()
+    torch.cuda.synchronize()
+    assert x[0].item() == 1 and cache.seq_pos == 600 and cache.num_blocks == 3
+    assert all(torch.equal(a, b) for a, b in zip(cache.get(torch.float32), before))
