@@ -72,6 +72,7 @@ use std::ffi::{c_char, c_int, c_void};
 pub type hs_stream_t = *mut c_void;
 
 pub const HS_ATTN_ABI_VERSION: c_int = @ABI@;
+pub const HS_ATTN_ABI_REVISION: c_int = @REVISION@;
 
 // enum hs_status
 pub const HS_OK: c_int = 0;
@@ -154,8 +155,11 @@ pub struct hs_qk_prologue {
 
 
 def main():
-    abi = re.search(r"#define\s+HS_ATTN_ABI_VERSION\s+(\d+)", open(os.path.join(HERE, "..", "include", "hs_attn.h")).read()).group(1)
-    out = HEAD.replace("@ABI@", abi)
+    header = open(os.path.join(HERE, "..", "include", "hs_attn.h")).read()
+    out = HEAD
+    for mark, name in (("@ABI@", "HS_ATTN_ABI_VERSION"), ("@REVISION@", "HS_ATTN_ABI_REVISION")):
+        number = re.search(r"#define\s+%s\s+(\d+)" % name, header).group(1)
+        out = out.replace(mark, number)
     out += '\n// ---- include/hs_attn.h -> libhs_attn.so\n#[link(name = "hs_attn")]\nextern "C" {\n%s\n}\n' % extern_block("hs_attn.h")
     out += ('\n// ---- include/hs_kv_cache.h -> libhs_kv_cache.so (optional host mirror)\n#[cfg(feature = "kv-cache")]\n'
             '#[link(name = "hs_kv_cache")]\nextern "C" {\n%s\n}\n' % extern_block("hs_kv_cache.h"))

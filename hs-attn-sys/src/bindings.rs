@@ -7,6 +7,7 @@ use std::ffi::{c_char, c_int, c_void};
 pub type hs_stream_t = *mut c_void;
 
 pub const HS_ATTN_ABI_VERSION: c_int = 8;
+pub const HS_ATTN_ABI_REVISION: c_int = 1;
 
 // enum hs_status
 pub const HS_OK: c_int = 0;
@@ -91,6 +92,7 @@ pub struct hs_qk_prologue {
 extern "C" {
     pub fn hs_attn_last_error() -> *const c_char;
     pub fn hs_attn_abi_version() -> c_int;
+    pub fn hs_attn_abi_revision() -> c_int;
     pub fn hs_kv_quantize_int8(k_src: *const c_void, v_src: *const c_void, src_dtype: c_int, k_codes: *mut i8, v_codes: *mut i8, k_scales: *mut f32, v_scales: *mut f32, layout: *const hs_kv_layout, positions: *const i32, start_pos: i32, b: i32, s: i32, hkv: i32, d: i32, stream: hs_stream_t) -> c_int;
     pub fn hs_kv_quantize_int8_rope(k_src: *const c_void, v_src: *const c_void, src_dtype: c_int, rope_sin: *const c_void, rope_cos: *const c_void, rope_len: i32, k_codes: *mut i8, v_codes: *mut i8, k_scales: *mut f32, v_scales: *mut f32, layout: *const hs_kv_layout, positions: *const i32, start_pos: i32, b: i32, s: i32, hkv: i32, d: i32, stream: hs_stream_t) -> c_int;
     pub fn hs_rope_apply(x: *const c_void, dtype: c_int, rope_sin: *const c_void, rope_cos: *const c_void, rope_len: i32, positions: *const i32, start_pos: i32, out: *mut c_void, b: i32, s: i32, h: i32, d: i32, stream: hs_stream_t) -> c_int;

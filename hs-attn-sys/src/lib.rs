@@ -39,13 +39,14 @@ pub fn check(rc: c_int) -> Result<()> {
     Err(HsAttnError { code: rc, message })
 }
 
-/// Refuses a library whose ABI differs from the one these bindings were generated for.
+/// Refuses a library whose ABI differs from the one these bindings were generated for, or that lacks what was added since
+/// (it would take a window for a reserved field and attend everything).
 pub fn check_abi() -> Result<()> {
-    let v = unsafe { bindings::hs_attn_abi_version() };
-    if v == bindings::HS_ATTN_ABI_VERSION {
+    let (v, r) = unsafe { (bindings::hs_attn_abi_version(), bindings::hs_attn_abi_revision()) };
+    if v == bindings::HS_ATTN_ABI_VERSION && r >= bindings::HS_ATTN_ABI_REVISION {
         Ok(())
     } else {
-        Err(HsAttnError { code: bindings::HS_ERR_INVALID_ARGUMENT, message: format!("libhs_attn ABI {v}, bindings {}", bindings::HS_ATTN_ABI_VERSION) })
+        Err(HsAttnError { code: bindings::HS_ERR_INVALID_ARGUMENT, message: format!("libhs_attn ABI {v}.{r}, bindings {}.{}", bindings::HS_ATTN_ABI_VERSION, bindings::HS_ATTN_ABI_REVISION) })
     }
 }
 

@@ -21,7 +21,7 @@ HS_ERR_BUSY = 6
 HS_BF16, HS_F32, HS_F16 = 0, 1, 2
 
 EXPORTS = [
-    "hs_attn_last_error", "hs_attn_abi_version",
+    "hs_attn_last_error", "hs_attn_abi_version", "hs_attn_abi_revision",
     "hs_kv_quantize_int8", "hs_kv_fp8_calibrate", "hs_kv_quantize_fp8", "hs_kv_dequantize",
     "hs_decode_attn_workspace_bytes", "hs_decode_attn_int8", "hs_decode_attn_fp8", "hs_decode_attn_phases",
     "hs_decode_step_int8", "hs_decode_step_fp8", "hs_prefill_attn_int8", "hs_prefill_attn_fp8", "hs_deltanet_forward",

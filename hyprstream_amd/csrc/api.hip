@@ -30,4 +30,6 @@ const char *hs_attn_last_error(void) { return hs::g_last_error; }
 
 int hs_attn_abi_version(void) { return HS_ATTN_ABI_VERSION; }
 
+int hs_attn_abi_revision(void) { return HS_ATTN_ABI_REVISION; }
+
 }  // extern "C"

@@ -47,6 +47,11 @@ extern "C" {
 #endif
 
 #define HS_ATTN_ABI_VERSION 8
+/* What has been added within the version: entry points, and fields in the place of reserved ones, which an older library
+ * of the same version takes for nothing.  1: attn_sinks, decode_window, hs_decode_step_weights, hs_attn_weights, hs_kv_evict.
+ * A caller that sets such a field asks for hs_attn_abi_revision() >= HS_ATTN_ABI_REVISION; libraries from before the first
+ * revision do not have the function, so it does not link or load with them. */
+#define HS_ATTN_ABI_REVISION 1
 
 typedef void *hs_stream_t; /* hipStream_t */
 
@@ -71,6 +76,7 @@ enum hs_dtype { HS_BF16 = 0, HS_F32 = 1, HS_F16 = 2 };
 
 struct hs_qk_prologue;
 
+/* Zero the whole struct, then set what is used: every optional field is off at zero. */
 typedef struct hs_kv_layout {
     int64_t code_stride_seq;    /* bytes between sequences (or blocks when paged) */
     int64_t code_stride_head;   /* bytes between kv-heads inside a sequence/block; >= capacity_tokens*D, multiple of 16 */
@@ -162,6 +168,7 @@ typedef struct hs_kv_layout {
 /* Message of the last failing call on this thread ("" if none). */
 HS_API const char *hs_attn_last_error(void);
 HS_API int hs_attn_abi_version(void);
+HS_API int hs_attn_abi_revision(void);
 
 /* ---- quantize-on-write (replaces the buffer + flush + requantize-everything scheme of
  * LayerKVCache::update / flush_buffer, kv_cache.rs:1275-1432, 1204-1272, and the

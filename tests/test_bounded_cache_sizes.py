@@ -1,10 +1,15 @@
-"""Workspaces sized once: for the longest call over a cache's capacity, used by every smaller one."""
+"""What callers of a bounded cache ask once: workspaces for the longest call over its capacity, used by every smaller one, and
+whether the library has windows at all."""
 import ctypes
+import os
 import random
+import re
 
 import pytest
 
 from hyprstream_amd import bindings as hb
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 P, CROOKED = ctypes.c_void_p(0x100000), ctypes.c_void_p(0x100040)
 
@@ -50,3 +55,14 @@ def test_the_bound_stays_near_what_calls_take(D):
     for B, S, G, Hkv, T in ((1, 1, 4, 8, 1 << 20), (1, 32, 4, 8, 32768), (4, 4096, 4, 8, 4096), (64, 1, 4, 8, 8192), (1, 32768, 8, 8, 32768), (64, 512, 1, 8, 8192)):
         n = hb.attn_weights_workspace_bytes(B, S, Hkv * G, Hkv, D, T)
         assert 4 * B * Hkv * S * G <= n <= 4 * B * Hkv * (S * G + 127) + (16 << 20)
+
+
+def test_revision_tells_libraries_with_windows_from_those_before():
+    """Windows took the place of reserved fields within one ABI version: the revision is what a caller of theirs asks for,
+    and a library from before does not have it."""
+    L, text = hb.lib(), open(os.path.join(ROOT, "include", "hs_attn.h")).read()
+    assert L.hs_attn_abi_revision() == int(re.search(r"#define HS_ATTN_ABI_REVISION (\d+)", text).group(1)) >= 1
+    rust = open(os.path.join(ROOT, "hs-attn-sys", "src", "bindings.rs")).read()
+    assert "pub const HS_ATTN_ABI_REVISION: c_int = %d;" % L.hs_attn_abi_revision() in rust
+    check = re.search(r"pub fn check_abi\(\).*?\n}", open(os.path.join(ROOT, "hs-attn-sys", "src", "lib.rs")).read(), flags=re.S).group(0)
+    assert "hs_attn_abi_revision()" in check and "HS_ATTN_ABI_REVISION" in check
