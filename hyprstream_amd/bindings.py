@@ -186,6 +186,18 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
+def _windowed(layout, field, window, sinks):
+    """The layout of one call: `field` and attn_sinks as the call names them, or as they are set on `layout` (None)."""
+    if window is None and sinks is None:
+        return layout
+    layout = KvLayout.from_buffer_copy(layout)
+    if window is not None:
+        setattr(layout, field, window)
+    if sinks is not None:
+        layout.attn_sinks = sinks
+    return layout
+
+
 def _dtype_code(t):
     import torch
     return {torch.bfloat16: HS_BF16, torch.float32: HS_F32, torch.float16: HS_F16}[t.dtype]
@@ -247,11 +259,11 @@ def kv_quantize_int8_prologue(k_src, v_src, prologue, k_codes, v_codes, k_scales
 
 
 def decode_step_prologue(q, k_new, v_new, prologue, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out,
-                         workspace, Hkv, max_seq_len, softmax_scale, fp8=False, window=0, sinks=0):
+                         workspace, Hkv, max_seq_len, softmax_scale, fp8=False, window=None, sinks=None):
     """decode_step (int8, or fp8 with calibrated scales) with the QK-norm and the rotation of q and k_new inside the
     launch.  window, sinks: as for decode_attn."""
     B, Hq, D = q.shape
-    layout.decode_window, layout.attn_sinks = window, sinks
+    layout = _windowed(layout, "decode_window", window, sinks)
     assert k_new.shape == (B, 1, Hkv, D) and k_new.is_contiguous() and v_new.is_contiguous()
     fn = lib().hs_decode_step_fp8_prologue if fp8 else lib().hs_decode_step_int8_prologue
     check(fn(_ptr(q), _ptr(k_new), _ptr(v_new), ctypes.byref(prologue), _ptr(k_codes), _ptr(v_codes), _ptr(k_scales),
@@ -289,11 +301,11 @@ def decode_workspace_bytes(B, Hq, Hkv, D, max_seq_len):
 
 
 def decode_attn(q, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, workspace, Hkv, max_seq_len,
-                softmax_scale, fp8=False, phases=3, window=0, sinks=0):
-    """window: the newest token attends the last `window` cached tokens (0 = all) and the first `sinks` ones
-    (layout.decode_window, layout.attn_sinks)."""
+                softmax_scale, fp8=False, phases=3, window=None, sinks=None):
+    """window: the newest token attends the last `window` cached tokens (0 = all) and the first `sinks` ones; None: as
+    layout.decode_window and layout.attn_sinks say."""
     B, Hq, D = q.shape
-    layout.decode_window, layout.attn_sinks = window, sinks
+    layout = _windowed(layout, "decode_window", window, sinks)
     if phases != 3:
         fn0 = lib().hs_decode_attn_phases
         fn = lambda *a: fn0(int(fp8), int(phases), *a)
@@ -306,21 +318,21 @@ def decode_attn(q, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, 
 
 
 def decode_attn_static(q, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, Hkv, max_seq_len, softmax_scale,
-                       window=0, sinks=0):
+                       window=None, sinks=None):
     """hs_decode_attn_int8 without a workspace argument: the split-K partials use the library's built-in scratch."""
     B, Hq, D = q.shape
-    layout.decode_window, layout.attn_sinks = window, sinks
+    layout = _windowed(layout, "decode_window", window, sinks)
     check(lib().hs_decode_attn_int8_static(_ptr(q), _ptr(k_codes), _ptr(v_codes), _ptr(k_scales), _ptr(v_scales),
                                            ctypes.byref(layout), _ptr(seq_lens), _ptr(out), B, Hq, Hkv, D,
                                            ctypes.c_int32(max_seq_len), ctypes.c_float(softmax_scale), _stream()))
 
 
 def decode_step(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, workspace, Hkv,
-                max_seq_len, softmax_scale, fp8=False, window=0, sinks=0):
+                max_seq_len, softmax_scale, fp8=False, window=None, sinks=None):
     """Quantize-on-write of one new token per sequence (at seq_lens-1) + decode attention, one call.  window, sinks: as
     for decode_attn."""
     B, Hq, D = q.shape
-    layout.decode_window, layout.attn_sinks = window, sinks
+    layout = _windowed(layout, "decode_window", window, sinks)
     assert k_new.shape == (B, 1, Hkv, D) and k_new.is_contiguous() and v_new.is_contiguous()
     fn = lib().hs_decode_step_fp8 if fp8 else lib().hs_decode_step_int8
     check(fn(q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), _dtype_code(k_new), k_codes.data_ptr(), v_codes.data_ptr(),
@@ -330,10 +342,10 @@ def decode_step(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, layout, s
 
 
 def decode_step_rope(q, k_new, v_new, rope_sin, rope_cos, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out,
-                     workspace, Hkv, max_seq_len, softmax_scale, window=0, sinks=0):
+                     workspace, Hkv, max_seq_len, softmax_scale, window=None, sinks=None):
     """decode_step (int8) with q and k_new arriving unrotated; bf16 tables [rope_len, D/2]."""
     B, Hq, D = q.shape
-    layout.decode_window, layout.attn_sinks = window, sinks
+    layout = _windowed(layout, "decode_window", window, sinks)
     assert k_new.shape == (B, 1, Hkv, D) and k_new.is_contiguous() and v_new.is_contiguous()
     check(lib().hs_decode_step_int8_rope(_ptr(q), _ptr(k_new), _ptr(v_new), _ptr(rope_sin), _ptr(rope_cos),
                                          ctypes.c_int32(rope_sin.shape[0]), _ptr(k_codes), _ptr(v_codes),
@@ -356,7 +368,7 @@ def _weights_rows(w_in, w_out, B, Hkv):
 
 
 def decode_step_weights(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, layout, seq_lens, out, weights_in, weights_out,
-                        workspace, Hkv, max_seq_len, softmax_scale, fp8=False, window=0, sinks=0):
+                        workspace, Hkv, max_seq_len, softmax_scale, fp8=False, window=None, sinks=None):
     """decode_step (decode_attn if k_new and v_new are None) and weights_out = weights_in + the softmax weights of the
     step summed over the query heads of each kv-head.  weights: fp32 [B, Hkv, stride]; weights_in may be None (zeros) or
     weights_out itself."""
@@ -364,7 +376,7 @@ def decode_step_weights(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, l
     assert q.is_contiguous() and out.is_contiguous()
     assert k_new is None or (k_new.shape == (B, 1, Hkv, D) and k_new.is_contiguous() and v_new.is_contiguous())
     stride = _weights_rows(weights_in, weights_out, B, Hkv)
-    layout.decode_window, layout.attn_sinks = window, sinks
+    layout = _windowed(layout, "decode_window", window, sinks)
     check(lib().hs_decode_step_weights(fp8, q.data_ptr(), _addr(k_new), _addr(v_new), HS_BF16 if k_new is None else _dtype_code(k_new),
                                        k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
                                        ctypes.addressof(layout), seq_lens.data_ptr(), out.data_ptr(), _addr(weights_in),
@@ -377,14 +389,14 @@ def attn_weights_workspace_bytes(B, S, Hq, Hkv, D, max_seq_len):
 
 
 def attn_weights(q, k_codes, k_scales, layout, weights_in, weights_out, workspace, Hkv, max_seq_len, softmax_scale,
-                 positions=None, start_pos=0, fp8=False, window=0, sinks=0):
+                 positions=None, start_pos=0, fp8=False, window=None, sinks=None):
     """weights_out = weights_in + the softmax weights of the queries q [B, S, Hq, D] (at (positions[b] or 0) + start_pos + s)
     over the cached keys, summed over queries and over the query heads of each kv-head."""
     B, S, Hq, D = q.shape
     assert q.is_contiguous() and str(q.dtype) == "torch.bfloat16"
     assert positions is None or (str(positions.dtype) == "torch.int32" and positions.is_contiguous() and positions.numel() == B)
     stride = _weights_rows(weights_in, weights_out, B, Hkv)
-    layout.prefill_window, layout.attn_sinks = window, sinks
+    layout = _windowed(layout, "prefill_window", window, sinks)
     check(lib().hs_attn_weights(fp8, q.data_ptr(), k_codes.data_ptr(), k_scales.data_ptr(), ctypes.addressof(layout), _addr(positions),
                                 start_pos, _addr(weights_in), weights_out.data_ptr(), stride, workspace.data_ptr(),
                                 workspace.numel() * workspace.element_size(), B, S, Hq, Hkv, D, max_seq_len, softmax_scale, _stream()))
@@ -442,13 +454,13 @@ PREFILL_COLUMNS = 0  # default for prefill_attn's `columns` (tests set it to run
 
 
 def prefill_attn(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, layout, hist_len, out, softmax_scale,
-                 quantize_on_write=True, fp8=False, hist_lens=None, columns=None, window=0, q_prologue=None,
-                 split_workspace=None, key_splits=0, shadow=None, sinks=0):
+                 quantize_on_write=True, fp8=False, hist_lens=None, columns=None, window=None, q_prologue=None,
+                 split_workspace=None, key_splits=0, shadow=None, sinks=None):
     """Causal attention of S new tokens over [int8 or fp8 history | their own bf16 K/V]; optionally caches them.
     hist_lens (int32 device tensor [B]): rows at different positions; hist_len is then their upper bound.
     columns: 0 = the library's choice of workgroup width, 256 or 128 fixes it (layout.prefill_columns_hint).
-    window: sliding window of local layers (layout.prefill_window), 0 = none; sinks: first tokens that stay visible
-    (layout.attn_sinks).
+    window: sliding window of local layers, 0 = none; sinks: first tokens that stay visible; None: as
+    layout.prefill_window and layout.attn_sinks say.
     q_prologue (QkPrologue): q arrives as projected and the launch normalises and rotates it
     (layout.prefill_q_prologue); k_new arrives normalised and rotated either way.
     split_workspace (uint8 device tensor from prefill_split_workspace()): lets a call with few query tiles split their
@@ -456,8 +468,8 @@ def prefill_attn(q, k_new, v_new, k_codes, v_codes, k_scales, v_scales, layout, 
     shadow ((uint8 device tensor, tokens) from prefill_shadow()): the bf16 operand-order copy of the prompt's K/V that
     every call appends to and calls with history read instead of the codes (layout.prefill_shadow)."""
     B, S, Hq, D = q.shape
+    layout = _windowed(layout, "prefill_window", window, sinks)
     layout.prefill_columns_hint = PREFILL_COLUMNS if columns is None else columns
-    layout.prefill_window, layout.attn_sinks = window, sinks
     layout.prefill_q_prologue = ctypes.addressof(q_prologue) if q_prologue is not None else None
     if split_workspace is None and key_splits == 0 and PREFILL_KEY_SPLITS > 1:
         key = (B, S, Hq, k_new.shape[2], D)
