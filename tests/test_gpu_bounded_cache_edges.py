@@ -7,6 +7,7 @@ import torch
 from hyprstream_amd import bindings as hb
 from hyprstream_amd import kv_cache as kc
 from bounded_util import Cache, DEV, bf16_randn
+from test_gpu_output_gate import _check as _check_gate, _with_gate
 
 pytestmark = pytest.mark.gpu
 
@@ -360,3 +361,24 @@ def test_paged_eviction_is_refused_under_capture():
     torch.cuda.synchronize()
     assert x[0].item() == 1 and cache.seq_pos == 600 and cache.num_blocks == 3
     assert all(torch.equal(a, b) for a, b in zip(cache.get(torch.float32), before))
+
+
+@pytest.mark.parametrize("B,T,D,fp8,window", [(1, 5000, 128, False, 0), (64, 300, 64, False, 0), (2, 3000, 256, True, 700), (70, 200, 128, True, 90)])
+def test_decode_weights_with_an_output_gate(B, T, D, fp8, window):
+    """The gate of hs_decode_step_weights: applied once, by the attention kernel (one chunk) or by the merge beside the
+    weights (split sequences), and the weights know nothing of it."""
+    Hq, Hkv = 8, 8 if B >= 64 else 2
+    c = Cache(7500 + T, B, Hkv, T, D, fp8=fp8)
+    assert (hb.decode_num_chunks(B, Hkv, min(T, window + 300) if window else T) > 1) == (B < 64)
+    q = bf16_randn(7501, B, Hq, D)
+    gate = (2 * bf16_randn(7502, B, Hq, D).float()).to(torch.bfloat16)
+    seq = torch.randint(1, T + 1, (B,), generator=torch.Generator().manual_seed(B), dtype=torch.int32).to(DEV)
+    ws = _space(hb.decode_weights_workspace_bytes(B, Hq, Hkv, D, T))
+    outs, ws_out = [], []
+    for layout in (c.layout, _with_gate(c.layout, gate)):
+        out, w = torch.full((B, Hq, D), float("nan"), dtype=torch.bfloat16, device=DEV), torch.zeros(B, Hkv, (T + 3) // 4 * 4, device=DEV)
+        hb.decode_step_weights(q, None, None, *c.tensors, layout, seq, out, None, w, ws, Hkv, T, D ** -0.5, fp8=fp8, window=window, sinks=5)
+        outs.append(out)
+        ws_out.append(w)
+    _check_gate(outs[1], outs[0], gate)
+    assert torch.equal(*ws_out) and ws_out[0].any()
