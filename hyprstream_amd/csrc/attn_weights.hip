@@ -7,13 +7,15 @@
 // lse_c is needed before the first p and takes all of s, so s is computed twice: weights_stats_kernel walks the keys for
 // a block of columns and leaves (m, l) per column, weights_columns_kernel walks the columns for a block of keys and adds
 // up.  (weights_narrow_kernel does both where all columns fit a wavefront.)  Storing p in between instead would move S x T
-// values per query head.  Both products run on the matrix cores with
-// exact operands (the result is an fp32 tensor, and a rounded operand would show in it): codes are integers (int8) or
-// short floats (e4m3fn) that fp16 and bf16 hold exactly, q is bf16.  Each kernel keeps its stationary side in registers
-// and converts only there or once per workgroup: columns as fp16 in the first (the streamed codes take one byte permute
-// and one subtraction per two), keys as bf16 in the second (the streamed q is used as it lies).
-// 4 x 4096 queries of 32 heads on their own keys (550 GFLOP in both products): 358 + 300 us under the profiler, 597 a call,
-// 920 TFLOP/s; the second kernel takes 219 without its LDS operand reads, which share the LDS with the tiles' copies.
+// values per query head.  Both products run on the matrix cores, and the result is an fp32 tensor in which a rounded
+// operand would show: codes are integers (int8) or short floats (e4m3fn) that fp16 and bf16 hold exactly, q is bf16.  Each
+// kernel keeps its stationary side in registers and converts only there or once per workgroup: columns in the first, keys
+// as bf16 in the second (the streamed q is used as it lies; the narrow kernels multiply bf16 by bf16 in both).  The first
+// kernel's columns are fp16 relative to a power of two P above their largest element (by 2 at most; by 2^5 where columns
+// share it), so that the streamed codes take one byte permute and one subtraction per two: bf16's eight bits fit down to
+// 2^-17 P, smaller elements are fp16 subnormals and off by at most 2^-25 P.
+// 4 x 4096 queries of 32 heads on their own keys (550 GFLOP in both products): 302 + 267 + 5 us, 575 a call, 956 TFLOP/s; the
+// second kernel takes 28 % less without its LDS operand reads, which share the LDS with the tiles' copies.
 // The keys sit on the M axis, so a lane's four score registers are four keys of one column: row statistics stay in the
 // lane until the end of the walk, and so do the column sums.
 #include <algorithm>
@@ -717,7 +719,7 @@ __global__ __launch_bounds__(kWThreads, 2) void weights_columns_kernel(WeightsAr
         if (a.segments == 1 && a.in && li == 0) before[u] = *(const float4v *)(a.in + (int64_t)unit * a.stride + min((int64_t)(wk0 + 16 * u + 4 * lq), a.stride - 4));
     }
     if (c_lo < c_hi) {
-        // ---- columns, kCStep a step: copy i of this thread is piece (x % CPR) of the tile's column x / CPR, x = tid + 512 i.
+        // ---- columns, kCStep a step: copy i of this thread is piece (x % CPR) of the tile's column x / CPR, x = tid + kWThreads i.
         //      Where kCStep is a multiple of G the columns' rows move by one constant from step to step.
         const float *lse = a.lse + (int64_t)unit * a.lse_stride;
         const uint8_t *qb = (const uint8_t *)(a.q + ((int64_t)b * a.S * a.Hq + h * a.G) * D);

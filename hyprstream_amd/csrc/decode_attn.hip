@@ -35,9 +35,9 @@
 // HBM bytes per cached token and kv-head: 2*D codes + 8 B of scales (int8) -- 264 B at D = 128.
 //
 // With a sliding window and sinks (kMode 1) only the visible tokens count, in those bytes as in the split: 64 ragged
-// sequences of up to 8192 tokens with a window of 4096 (555 MB) take 85 us, 6.5 TB/s; one of 32768 with a window of 1024
-// takes 8.3 + 3.4 us, the latency of a 256-token chunk and of the merge.  With the step's softmax weights (kMode 2) the
-// scores pass through memory as well, 4 bytes per head and token each way: 64 x 8192 take 205 us (173 plain) and 19 us for
+// sequences of up to 8192 tokens with a window of 4096 (555 MB) take 84 us, 6.6 TB/s; one of 32768 with a window of 1024
+// takes 8.5 + 3.9 us, the latency of a 256-token chunk and of the merge.  With the step's softmax weights (kMode 2) the
+// scores pass through memory as well, 4 bytes per head and token each way: 64 x 8192 take 197 us (173 plain) and 18 us for
 // the weights, 1142 MB in 216 us a call.
 #include <atomic>
 #include <mutex>

@@ -7,8 +7,10 @@
 // parallel; evict_inplace_kernel does the same inside one buffer, where a tile may only be overwritten once it has been
 // read, with one workgroup per (sequence, kv-head, tensor) that walks its tiles in order.
 //
-// 64 x 8 rows of 8192 tokens cut to 1024 (D = 128; 300 MB of weights, kept rows read and written): 14 us of selection and 54
-// of copy at 5.3 TB/s.  8 rows of 32768 cut to 4096: 22 us, one workgroup's chain of passes over a row, and 5 of copy.
+// 64 x 8 rows of 8192 tokens cut to 1024 (D = 128; 300 MB of weights, kept rows read and written): 14 us of selection and 53
+// of copy at 5.3 TB/s.  8 rows of 32768 cut to 4096: 23 us, one workgroup's chain of passes over a row, and 4 of copy.
+// Caches and weights flushed by other work before every call: 92 us for the first (in place 90), 39 for the second (in place
+// 73: two workgroups a row walk its tiles in order), 8 rows of 131072 cut to 16384 153 (in place 300).
 #include <algorithm>
 #include <type_traits>
 
@@ -33,7 +35,7 @@ struct EvictArgs {
     int32_t *kept;      // caller's list or nullptr
     int32_t *list;      // workspace [B, Hkv, budget]
     int32_t *info;      // workspace [B, Hkv, 2]: tokens kept, first list entry that moves
-    int32_t budget, sinks, recent, Hkv, D, max_seq_len, fp8;
+    int32_t budget, sinks, recent, Hkv, max_seq_len, fp8;
     int32_t finish;     // entries per row of kept and weights_out that are written
 };
 
@@ -514,7 +516,7 @@ int hs_kv_evict(int fmt_fp8, const void *k_codes, const void *v_codes, const flo
     a.list = (int32_t *)workspace;
     a.info = a.list + (size_t)B * Hkv * budget;
     a.budget = budget; a.sinks = sinks; a.recent = recent;
-    a.Hkv = Hkv; a.D = D; a.max_seq_len = max_seq_len; a.fp8 = fp8 ? 1 : 0;
+    a.Hkv = Hkv; a.max_seq_len = max_seq_len; a.fp8 = fp8 ? 1 : 0;
     a.finish = std::max(std::min(budget, max_seq_len), kept ? budget : 0);
     if (weights_out) a.finish = std::max<int64_t>(a.finish, std::min<int64_t>(weights_out_stride, max_seq_len));
     hipStream_t st = (hipStream_t)stream;
