@@ -77,10 +77,10 @@ Status BlockPool::await(BlockId id, hs_stream_t stream, bool *clear) {
     auto &f = fence_[(size_t)id];
     *clear = !f;
     if (*clear) return {};
-    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
-    if (hipError_t e = hipStreamIsCapturing((hipStream_t)stream, &capturing); e != hipSuccess) return hip_err(e, "asking for a capture");
-    if (capturing != hipStreamCaptureStatusNone)
-        return err(HS_ERR_BUSY, "a block comes from an eviction that is still queued: make one call with it before the capture");
+    bool capturing = false;
+    if (hipError_t e = is_capturing((hipStream_t)stream, &capturing); e != hipSuccess) return hip_err(e, "asking for a capture");
+    if (capturing)
+        return err(HS_ERR_BUSY, "a block comes from an eviction: once that has run, make a call with the block before the capture");
     hipError_t e = hipEventQuery(f->event);
     if (e == hipSuccess) {
         f.reset();
@@ -348,9 +348,9 @@ Status PagedLayerKVCache::evict(float *weights, int64_t weights_stride, int32_t 
     if (budget <= 0 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
         return err(HS_ERR_INVALID_ARGUMENT, "need budget > 0 and 0 <= sinks + recent <= budget");
     if ((size_t)budget >= seq_pos) return {};
-    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
-    if (hipError_t e = hipStreamIsCapturing((hipStream_t)stream, &capturing); e != hipSuccess) return hip_err(e, "asking for a capture");
-    if (capturing != hipStreamCaptureStatusNone)
+    bool capturing = false;
+    if (hipError_t e = is_capturing((hipStream_t)stream, &capturing); e != hipSuccess) return hip_err(e, "asking for a capture");
+    if (capturing)
         return err(HS_ERR_INVALID_ARGUMENT, "a paged cache is not evicted under stream capture: its blocks go back to the pool once");
     if (Status s = sync_table(stream); !s.ok()) return s;
     const int32_t heads = pool_->num_kv_heads(), dim = pool_->head_dim(), len = (int32_t)seq_pos;

@@ -19,6 +19,15 @@ inline hipError_t fill_i32(int32_t *p, int32_t n, int32_t v, hipStream_t stream)
     return hipGetLastError();
 }
 
+// Is `stream` being captured?  (On an error that one is given back, and not left to the next launch's check.)
+inline hipError_t is_capturing(hipStream_t stream, bool *yes) {
+    hipStreamCaptureStatus s = hipStreamCaptureStatusNone;
+    const hipError_t e = hipStreamIsCapturing(stream, &s);
+    if (e != hipSuccess) (void)hipGetLastError();
+    *yes = s != hipStreamCaptureStatusNone;
+    return e;
+}
+
 // Columns [from, to) of `rows` rows of `stride` floats.
 static __global__ void zero_columns_kernel(float *p, int64_t rows, int64_t stride, int64_t from, int64_t to) {
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, n = to - from;

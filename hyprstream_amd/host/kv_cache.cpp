@@ -184,6 +184,10 @@ Status LayerKVCache::evict(int32_t budget, int32_t sinks, int32_t recent, hs_str
     if (budget <= 0 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > budget)
         return err(HS_ERR_INVALID_ARGUMENT, "need budget > 0 and 0 <= sinks + recent <= budget");
     if ((size_t)budget >= seq_pos) return {};
+    bool capturing = false;
+    if (hipError_t e = is_capturing((hipStream_t)stream, &capturing); e != hipSuccess) return hip_err(e, "asking for a capture");
+    if (capturing)
+        return err(HS_ERR_INVALID_ARGUMENT, "a cache is not evicted under stream capture: its position moves once, the tokens at every replay");
     if (Status s = ensure_weights(0, 0, stream); !s.ok()) return s;
     if (Status s = set_lengths(stream); !s.ok()) return s;
     const int rc = hs_kv_evict(quant_type_ == KVQuantType::Fp8, k_codes_, v_codes_, k_scales_, v_scales_, &layout_, seq_lens_dev_, weights_,

@@ -112,7 +112,8 @@ HS_API int hs_cache_prefill(hs_cache *c, const void *q, const void *new_keys, co
  * hs_cache_get_weights: the entries as dense [batch, num_kv_heads, seq_pos], copied on `stream`.
  * hs_cache_evict: keeps `budget` tokens per (sequence, kv-head) -- the first `sinks`, the last `recent` and the heaviest of
  *   those between; without tracking the first `sinks` and the newest -- in place (hs_kv_evict).  seq_pos becomes
- *   min(seq_pos, budget).  Keys keep their rotation: rotate later tokens by their true position, not by seq_pos. */
+ *   min(seq_pos, budget).  Keys keep their rotation: rotate later tokens by their true position, not by seq_pos.  Refused
+ *   under stream capture: seq_pos would move once, the tokens at every replay (hs_kv_evict itself can be captured). */
 HS_API int hs_cache_set_window(hs_cache *c, int32_t window, int32_t sinks);
 HS_API int hs_cache_track_weights(hs_cache *c, int on);
 HS_API int hs_cache_get_weights(hs_cache *c, float *weights_out, hs_stream_t stream);

@@ -344,9 +344,48 @@ def test_blocks_of_a_queued_eviction_wait_for_it(taker):
         assert two.seq_pos == 257 and all(torch.equal(a, b) for a, b in zip(two.get(torch.float32), alone.get(torch.float32)))
 
 
-def test_paged_eviction_is_refused_under_capture():
+def test_capture_over_blocks_of_a_queued_eviction():
+    """A step over blocks that an eviction gave back is refused under capture until a plain call has seen the eviction end."""
+    Hq, Hkv, D = 4, 2, 64
+    pool = kc.BlockPool(8, Hkv, D, kc.INT8)
+    one, two = kc.PagedLayerKVCache(1024, pool, "one"), kc.PagedLayerKVCache(1024, pool, "two")
+    k, q = bf16_randn(7760, 1, 600, Hkv, D), bf16_randn(7761, 1, Hq, D)
+    two.update(k[:, :256], k[:, :256], 0)
+    one.update(k, k, 0)
+    one.evict(100)
+    x = torch.zeros(4, device=DEV)
+    torch.cuda.synchronize()
+
+    def capture(body):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+            body()
+        return g
+
+    def refused():
+        with pytest.raises(kc.CacheError, match="eviction") as e:
+            two.update(k[:, :1], k[:, :1], 256)
+        assert e.value.code == hb.HS_ERR_BUSY
+        x.add_(1)
+
+    capture(refused).replay()
+    assert two.seq_pos == 256
+    two.update(k[:, :1], k[:, :1], 256)
+    want, out = two.decode_attention(q, 0.125), torch.empty_like(q)
+    torch.cuda.synchronize()
+    g = capture(lambda: two._check(kc.lib().hs_paged_cache_decode_attention(two._h, hb._ptr(q), hb._ptr(out), Hq, ctypes.c_float(0.125), hb._stream())))
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and x[0].item() == 1
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_eviction_through_the_mirrors_is_refused_under_capture(paged):
+    """It moves a position and gives blocks back when it is called, tokens whenever the graph is replayed."""
     pool = kc.BlockPool(8, 2, 64, kc.INT8)
-    cache = kc.PagedLayerKVCache(1024, pool, "s")
+    cache = kc.PagedLayerKVCache(1024, pool, "s") if paged else kc.LayerKVCache(1024)
     k = bf16_randn(7750, 1, 600, 2, 64)
     cache.update(k, k, 0)
     before = [t.clone() for t in cache.get(torch.float32)]
@@ -359,7 +398,7 @@ def test_paged_eviction_is_refused_under_capture():
         x += 1
     g.replay()
     torch.cuda.synchronize()
-    assert x[0].item() == 1 and cache.seq_pos == 600 and cache.num_blocks == 3
+    assert x[0].item() == 1 and cache.seq_pos == 600 and pool.used_blocks() == (6 if paged else 0)
     assert all(torch.equal(a, b) for a, b in zip(cache.get(torch.float32), before))
 
 
