@@ -387,7 +387,7 @@ __global__ __launch_bounds__(256, 2) void decode_attn_kernel(DecodeArgs a_in) {
     const int li = lane & 15, lq = lane >> 4;
     __shared__ __attribute__((aligned(16))) float sm_sc[kWavesPerWg][64 * NS];
     __shared__ float sm_m[kWavesPerWg][16], sm_l[kWavesPerWg][16];
-    __shared__ float sm_o[kWavesPerWg][16][CW + 4];  // one column group of O at a time
+    __shared__ __attribute__((aligned(16))) float sm_o[kWavesPerWg][16][CW + 4];  // one column group of O at a time (kMode 2: read and written 16 bytes at a time)
     // One work item: tokens [t_begin, t_end) of sequence b (L cached tokens), partial slot `chunk`.  (kMode >= 1: t_begin
     // and t_end count on the visible line, `line`.)
     struct Item {
